@@ -7,4 +7,6 @@ reference's `Srgemm` / `SrgemmSplitKParallel` host operators used by the tests a
 from .semiring import DType, Layout, Op, RINGS, Status, annihilator, identity  # noqa: F401
 from .srgemm import (Arguments, Srgemm, SrgemmSplitKParallel, STATIC_SCRATCH_BYTES, device_status,  # noqa: F401
                      launch_count, pack_k_contiguous, srgemm_path, srgemm_splitk_static)
+from .decode import (BeamArguments, BeamStep, Q4Arguments, Q4Product, ReorderArguments, ReorderStates,  # noqa: F401
+                     StateView, state_view)
 from .host_pipeline import HostSrgemm  # noqa: F401,E402

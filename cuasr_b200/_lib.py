@@ -72,6 +72,54 @@ class ApspMultiArgs(ctypes.Structure):     # cuasr_b200_apsp_multi_args_t
     ]
 
 
+class Q4Args(ctypes.Structure):            # cuasr_b200_q4_args_t
+    _fields_ = [
+        ("dtype_x", ctypes.c_int32), ("dtype_y", ctypes.c_int32), ("dtype_scale", ctypes.c_int32), ("group", ctypes.c_int32),
+        ("m", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("device", ctypes.c_int32),
+        ("X", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+        ("W", ctypes.c_void_p), ("ldw", ctypes.c_int64),
+        ("scales", ctypes.c_void_p), ("ld_scales", ctypes.c_int64),
+        ("zeros", ctypes.c_void_p), ("ld_zeros", ctypes.c_int64),
+        ("Y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class BeamArgs(ctypes.Structure):          # cuasr_b200_beam_args_t
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("normalise", ctypes.c_int32),
+        ("batch", ctypes.c_int32), ("beams", ctypes.c_int32), ("vocab", ctypes.c_int32), ("keep", ctypes.c_int32),
+        ("end_token", ctypes.c_int32), ("device", ctypes.c_int32),
+        ("logits", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("beam_stride", ctypes.c_int64),
+        ("scores", ctypes.c_void_p), ("ld_scores", ctypes.c_int64),
+        ("finished", ctypes.c_void_p), ("ld_finished", ctypes.c_int64),
+        ("out_scores", ctypes.c_void_p), ("ld_out_scores", ctypes.c_int64),
+        ("parents", ctypes.c_void_p), ("ld_parents", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p), ("ld_tokens", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class State(ctypes.Structure):             # cuasr_b200_state_t
+    _fields_ = [
+        ("src", ctypes.c_void_p), ("dst", ctypes.c_void_p),
+        ("src_batch", ctypes.c_int64), ("src_beam", ctypes.c_int64), ("src_segment", ctypes.c_int64), ("src_position", ctypes.c_int64),
+        ("dst_batch", ctypes.c_int64), ("dst_beam", ctypes.c_int64), ("dst_segment", ctypes.c_int64), ("dst_position", ctypes.c_int64),
+        ("bytes", ctypes.c_int64), ("segments", ctypes.c_int32), ("positions", ctypes.c_int32),
+        ("ragged", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class ReorderArgs(ctypes.Structure):       # cuasr_b200_reorder_args_t
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("beams", ctypes.c_int32), ("keep", ctypes.c_int32), ("n_states", ctypes.c_int32),
+        ("parents", ctypes.c_void_p), ("ld_parents", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+        ("states", ctypes.POINTER(State)), ("device", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/*.h declares
 PROTOTYPES = {
     "cuasr_b200_srgemm_can_implement": (ctypes.c_int, [ctypes.POINTER(Desc), ctypes.POINTER(Args)]),
@@ -101,6 +149,13 @@ PROTOTYPES = {
     "cuasr_b200_pack_k_contiguous": (ctypes.c_int, [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
                                                     ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
                                                     ctypes.c_void_p]),
+    "cuasr_b200_q4_product_can_implement": (ctypes.c_int, [ctypes.POINTER(Q4Args)]),
+    "cuasr_b200_q4_product": (ctypes.c_int, [ctypes.POINTER(Q4Args)]),
+    "cuasr_b200_beam_step_can_implement": (ctypes.c_int, [ctypes.POINTER(BeamArgs)]),
+    "cuasr_b200_beam_step_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(BeamArgs)]),
+    "cuasr_b200_beam_step": (ctypes.c_int, [ctypes.POINTER(BeamArgs)]),
+    "cuasr_b200_reorder_states_can_implement": (ctypes.c_int, [ctypes.POINTER(ReorderArgs)]),
+    "cuasr_b200_reorder_states": (ctypes.c_int, [ctypes.POINTER(ReorderArgs)]),
     "cuasr_b200_device_status": (ctypes.c_int, [ctypes.c_void_p]),
     "cuasr_b200_last_kernel": (ctypes.c_char_p, []),
     "cuasr_b200_last_route": (ctypes.c_char_p, []),

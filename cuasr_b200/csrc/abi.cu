@@ -15,6 +15,7 @@
 
 #include "../../include/cuasr_b200.h"
 #include "../../include/cuasr_b200_apsp.h"
+#include "decode_launch.h"
 #include "srgemm_launch.h"
 #include "srgemm_path.cuh"
 #include "srgemm_screened.cuh"
@@ -988,6 +989,21 @@ cudaError_t static_scratch_address(void** out) {
 }
 
 }  // namespace
+
+bool current_device_info(DeviceInfo* out) {
+  DeviceState* dev = nullptr;
+  if (!device_state(&dev)) return false;
+  *out = {dev->sms, dev->status};
+  return true;
+}
+
+void note_launches(const char* kernel, int count) {
+  t_last_kernel = kernel;
+  t_route = Route();
+  t_route.kernel = kernel;
+  g_launches.fetch_add(static_cast<uint64_t>(count));
+}
+
 }  // namespace cuasr_b200
 
 using namespace cuasr_b200;

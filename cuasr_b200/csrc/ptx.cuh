@@ -18,6 +18,7 @@ enum DeviceStatus : unsigned int {
   kDeviceTimeoutFull     = 1,  // a consumer gave up waiting for a tile to land in shared memory
   kDeviceTimeoutEmpty    = 2,  // the producer gave up waiting for a stage to be released
   kDeviceTimeoutPeerFlag = 3,  // a rank gave up waiting for a peer's arrival flag
+  kDeviceIndexOutOfRange = 4,  // an index read from memory was outside its range and was not followed
 };
 
 __device__ __forceinline__ void report_device_error(unsigned int* status, unsigned int code) {

@@ -29,6 +29,8 @@ class DType(enum.IntEnum):
     F64 = 1
     S32 = 2
     U32 = 3
+    F16 = 4    # the decoding operators alone (decode.py)
+    BF16 = 5
 
 
 class Layout(enum.IntEnum):

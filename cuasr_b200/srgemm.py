@@ -74,6 +74,8 @@ class _Operator:
                  layout_c: Layout = Layout.COLUMN_MAJOR, split_k_serial: bool = False,
                  add_identity=None, mul_identity=None):
         self.add_op, self.mul_op, self.dtype = Op(add_op), Op(mul_op), DType(dtype)
+        if self.dtype not in _PACK_SCALAR:
+            raise ValueError(f"no semiring product takes {self.dtype!r}")
         self.layout_a, self.layout_b, self.layout_c = Layout(layout_a), Layout(layout_b), Layout(layout_c)
         self.kSplitKSerial = bool(split_k_serial)
         # AdditionOp::Identity / MultiplicationOp::Identity of the functors the operator is "instantiated" with

@@ -175,7 +175,8 @@ CUASR_B200_API int cuasr_b200_pack_k_contiguous(int32_t dtype, const void *src, 
 
 /* Reads (and clears) the device-side status word of the current device after synchronising `stream`:
  * 0 = every kernel of this library ran to completion; otherwise a bounded wait inside a kernel expired
- * (1: tile never arrived, 2: stage never released, 3: peer flag never set).  This call blocks. */
+ * (1: tile never arrived, 2: stage never released, 3: peer flag never set), or a kernel met an index outside its range
+ * and did not follow it (4: cuasr_b200_reorder_states, cuasr_b200_decode.h).  This call blocks. */
 CUASR_B200_API int cuasr_b200_device_status(void *stream);
 
 /* A label for the last cuasr_b200_srgemm* call on this thread that depends on its arguments alone: "tma...", "path_tma" where

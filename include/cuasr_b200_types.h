@@ -32,7 +32,10 @@ typedef enum cuasr_dtype {
   CUASR_F32 = 0,
   CUASR_F64 = 1,
   CUASR_S32 = 2,
-  CUASR_U32 = 3
+  CUASR_U32 = 3,
+  /* 16-bit types of the decoding operators (cuasr_b200_decode.h); no semiring product takes them. */
+  CUASR_F16  = 4, /* IEEE binary16 */
+  CUASR_BF16 = 5  /* the upper half of a binary32 */
 } cuasr_dtype_t;
 
 /* cutlass::layout::{ColumnMajor,RowMajor}; one leading dimension in elements. */
