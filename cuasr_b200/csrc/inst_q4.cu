@@ -1,31 +1,116 @@
-// Launcher of the products with 4-bit weights.
+// Plans and launches the products with 4-bit weights.
+#include <algorithm>
+
 #include "decode_launch.h"
-#include "q4_product.cuh"
-#include "srgemm_launch.h"
+#include "q4_launch.cuh"
 namespace cuasr_b200 {
-template <typename TX, typename TY, typename TS>
-static cudaError_t launch(const cuasr_b200_q4_args_t& a, int* launches) {
-  Q4Params p = {a.X, a.ldx, a.W, a.ldw, a.scales, a.ld_scales, a.zeros, a.ld_zeros, a.Y, a.ldy, a.m, a.n, a.k, a.group,
-                static_cast<int>((static_cast<long long>(a.k) + a.group - 1) / a.group)};
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((a.n + 7) / 8, (a.m + 3) / 4);
-  config.blockDim = dim3(256);
-  config.stream = static_cast<cudaStream_t>(a.stream);
-  *launches = 1;
-  return cudaLaunchKernelEx(&config, q4_rows_kernel<TX, TY, TS>, p);
+namespace {
+
+struct Q4Plan {
+  int parts = 0, slices = 1, panel_steps = 0, stages = 0, grid = 0, sum_bytes = 0, xsum_bytes = 0, smem = 0;
+};
+// What the shape of X and of the groups makes of a block.
+struct Q4Shape {
+  int columns, column_tiles, warps, groups_per_step, stage_bytes;
+};
+
+// Shared memory of a block: stages, sums, X of a panel and what is read behind it.
+void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
+  plan->sum_bytes = s.warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * kQ4SumStride * 4;
+  const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = s.warps * s.stage_bytes;
+  const int per_step = 512 * s.columns + 4 * s.groups_per_step * ((s.columns + 1) / 2 * 2), room = kQ4SmemPerBlock - fixed;
+  int panel = slice_steps;
+  if (panel > (room - 2 * all_stages) / per_step) panel = (room - 2 * all_stages) / per_step / plan->parts * plan->parts;
+  plan->panel_steps = panel;
+  plan->stages = 2;                  // three measured slower: 128000 x 4096 read alone in 53 us instead of 45
+  plan->xsum_bytes = (4 * s.groups_per_step * ((s.columns + 1) / 2 * 2) * panel + 15) / 16 * 16;
+  plan->smem = fixed - 16 + plan->xsum_bytes + panel * 512 * s.columns + plan->stages * all_stages;
 }
-template <typename TX, typename TY>
-static cudaError_t by_scale(const cuasr_b200_q4_args_t& a, int* launches) {
-  if (a.dtype_scale == CUASR_F32) return launch<TX, TY, float>(a, launches);
-  return a.dtype_scale == CUASR_F16 ? launch<TX, TY, __half>(a, launches) : launch<TX, TY, __nv_bfloat16>(a, launches);
+
+Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, int sms) {
+  Q4Plan best;
+  double best_cost = 0;
+  for (int parts = 1; parts <= shape.warps && parts <= 8; parts *= 2)
+    for (int s = 1; s <= kQ4MaxSlices && (s == 1 || s <= steps); s *= 2) {
+      Q4Plan plan;
+      plan.parts = parts;
+      plan.slices = s;
+      const int workers = shape.warps / parts, slice_steps = (steps + s - 1) / s;
+      fit(&plan, slice_steps, shape);
+      if (plan.panel_steps <= 0) continue;
+      const int blocks = std::max(1, std::min((units + workers - 1) / workers, std::max(1, sms / s)));
+      const double rounds = static_cast<double>(((units + workers - 1) / workers + blocks - 1) / blocks) * passes;
+      // In microseconds, from measurements between 1024 x 1024 and 128000 x 4096: a warp's step 1.7 with all warps at it, a
+      // worker's sums 1.3, a cluster's 2 more; X laid out by a block 0.5 for a step of all its columns' warps.  (One row,
+      // 14336 x 4096: 12.4 with four parts, 13.9 with eight, 17 with two.  Eight rows, 128000 x 4096: 63 with one part, 65 with
+      // four.  Thirty-two rows, 8192 x 8192: 38 with four slices of one part, 48 with two of two, 84 with two parts alone.)
+      const double restaged = plan.panel_steps < slice_steps ? rounds : passes;
+      const double cost = rounds * ((slice_steps + parts - 1) / parts * 1.7 + (parts > 1 ? 1.3 : 1.0) + (s > 1 ? 2.0 : 0.0)) +
+                          restaged * slice_steps * shape.columns * 0.5 / shape.warps;
+      if (best.smem == 0 || cost < best_cost) {
+        best_cost = cost;
+        plan.grid = blocks * s;
+        best = plan;
+      }
+    }
+  return best;
 }
-template <typename TX>
-static cudaError_t by_y(const cuasr_b200_q4_args_t& a, int* launches) {
-  if (a.dtype_y == CUASR_F32) return by_scale<TX, float>(a, launches);
-  return a.dtype_y == CUASR_F16 ? by_scale<TX, __half>(a, launches) : by_scale<TX, __nv_bfloat16>(a, launches);
+
+// Weight rows as bytes: boxes of 32 rows by the 64 bytes of half a step; zeros outside.
+bool weight_map(CUtensorMap* map, const cuasr_b200_q4_args_t& a) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (encode == nullptr || reinterpret_cast<uintptr_t>(a.W) % 16 != 0 || a.ldw % 16 != 0 || a.ldw >= (1LL << 40)) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>((static_cast<int64_t>(a.k) + 1) / 2), static_cast<cuuint64_t>(a.n)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.ldw)};
+  const cuuint32_t box[2] = {kQ4Step / 4, kQ4Rows}, ones[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(a.W), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo&, int* launches) {
-  if (a.dtype_x == CUASR_F32) return by_y<float>(a, launches);
-  return a.dtype_x == CUASR_F16 ? by_y<__half>(a, launches) : by_y<__nv_bfloat16>(a, launches);
+
+}  // namespace
+
+cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int* launches) {
+  Q4Params p = {};
+  p.X = a.X; p.ldx = a.ldx; p.W = a.W; p.ldw = a.ldw; p.scales = a.scales; p.ld_scales = a.ld_scales;
+  p.zeros = a.zeros; p.ld_zeros = a.ld_zeros; p.Y = a.Y; p.ldy = a.ldy;
+  p.m = a.m; p.n = a.n; p.k = a.k; p.group = a.group;
+  p.groups = static_cast<int>((static_cast<long long>(a.k) + a.group - 1) / a.group);
+  p.group_shift = -1;
+  for (int b = 5; b < 31; ++b)
+    if (a.group == 1 << b) p.group_shift = b;
+  p.type_x = a.dtype_x; p.type_y = a.dtype_y; p.type_scale = a.dtype_scale;
+  p.status = dev.status;
+  // offsets inside a tile are 32-bit
+  if (a.ld_scales > (1 << 24) || a.ld_zeros > (1 << 24) || a.n > 0x7FFFFFFF - 1024 || a.k > 0x7FFFFFFF - kQ4Step) return cudaErrorInvalidConfiguration;
+  const int parts = a.dtype_x == CUASR_F32 ? 3 : 1, most_rows = 32 / parts;
+  const int passes = (a.m - 1) / most_rows + 1;
+  if (passes > 65535) return cudaErrorInvalidConfiguration;
+  p.rows = (a.m - 1) / passes + 1;
+  const int columns = p.rows * parts, nt = columns <= 8 ? 1 : columns <= 16 ? 2 : 4;
+  const size_t es = a.dtype_x == CUASR_F32 ? 4 : 2;
+  p.x_vectors = reinterpret_cast<uintptr_t>(a.X) % 16 == 0 && (a.ldx * es % 16 == 0 || a.m == 1);
+  const int lw = a.group % 128 == 0 || a.group >= a.k ? 4 : a.group % 64 == 0 ? 2 : 1;
+  const int steps = (a.k + kQ4Step - 1) / kQ4Step;
+  CUtensorMap map = {};
+  const bool tma = weight_map(&map, a);
+  const Q4Shape shape = {columns, nt, nt == 4 ? kQ4Warps<4> : kQ4Warps<1>, 8 / lw, tma ? kQ4Stage<true> : kQ4Stage<false>};
+  p.units = (a.n - 1) / kQ4Rows + 1;
+  const Q4Plan plan = plan_q4(p.units, steps, passes, shape, dev.sms);
+  if (plan.smem == 0) return cudaErrorInvalidValue;      // no launch fits: never for one block per SM and one slice
+  p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.stages = plan.stages; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
+  const Q4Launch l = {plan.grid, passes, plan.smem, static_cast<cudaStream_t>(a.stream)};
+  const cudaError_t err = nt == 1   ? launch_q4_columns<1>(lw, tma, map, p, l)
+                          : nt == 2 ? launch_q4_columns<2>(lw, tma, map, p, l)
+                                    : launch_q4_columns<4>(lw, tma, map, p, l);
+  if (err == cudaSuccess) ++*launches;
+  return err;
 }
+
 }  // namespace cuasr_b200

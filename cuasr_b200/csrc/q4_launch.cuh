@@ -1,0 +1,69 @@
+// Launchers of q4_kernel; instantiated by the number of columns in the inst_q4_*.cu files so that they compile in parallel.
+#pragma once
+
+#include <atomic>
+
+#include "q4_product.cuh"
+
+namespace cuasr_b200 {
+
+// a block has 1 KB of static shared memory and 1 KB that the driver keeps
+constexpr int kQ4SmemPerSm = 228 * 1024, kQ4SmemPerBlock = kQ4SmemPerSm - 2048;
+
+// Opts a kernel in to more than 48 KB of shared memory, once per device.
+inline cudaError_t allow_shared_memory(const void* kernel, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemPerBlock);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return err;
+}
+
+struct Q4Launch {
+  int grid_x, grid_y, smem;
+  cudaStream_t stream;
+};
+
+template <bool BF16, int NT, int LW, bool TMA, bool ZEROS>
+cudaError_t launch_q4_kernel(const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
+  static std::atomic<uint64_t> allowed{0};
+  auto kernel = q4_kernel<BF16, NT, LW, TMA, ZEROS>;
+  const cudaError_t err = allow_shared_memory(reinterpret_cast<const void*>(kernel), allowed);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(l.grid_x), static_cast<unsigned>(l.grid_y));
+  config.blockDim = dim3(32 * kQ4Warps<NT>);
+  config.dynamicSmemBytes = static_cast<size_t>(l.smem);
+  config.stream = l.stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.slices);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = p.slices > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, kernel, map, p);
+}
+
+template <int NT>
+cudaError_t launch_q4_columns(int lw, bool tma, const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
+  const bool zeros = p.zeros != nullptr, bf16 = p.type_x != CUASR_F16;
+#define Q4_CASE(L, V, Z)                                                            \
+  if (lw == L && tma == V && zeros == Z)                                            \
+    return bf16 ? launch_q4_kernel<true, NT, L, V, Z>(map, p, l) : launch_q4_kernel<false, NT, L, V, Z>(map, p, l);
+#define Q4_CASES(L) Q4_CASE(L, false, false) Q4_CASE(L, true, false) Q4_CASE(L, false, true) Q4_CASE(L, true, true)
+  Q4_CASES(1) Q4_CASES(2) Q4_CASES(4)
+#undef Q4_CASES
+#undef Q4_CASE
+  return cudaErrorInvalidValue;
+}
+
+extern template cudaError_t launch_q4_columns<1>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<2>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<4>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+
+}  // namespace cuasr_b200

@@ -1,9 +1,52 @@
-// Plus-times product of a few rows with weights in 4 bits.
+// Plus-times product of a few rows with weights in 4 bits: Y = X W^T, W = scale (q - zero) by groups along k.
+//
+// The weights are read once, so the floor is their bytes at the memory's rate; at 6.5 TB/s that is 46 weights per SM and
+// clock, which leaves about ten instructions of a lane for eight weights.  Hence the tensor cores do the products
+// (mma.sync m16n8k16: sixteen weight rows by up to eight rows of X; an eighth of a tile is enough for one row, and the
+// instruction is not what bounds the kernel), and four bits become a factor by a single AND.  As the last bits of a 16-bit
+// number they are the subnormal q u, four places further up 16 q u, both exact (u = 2^-24 in binary16; 2^-133 in bfloat16,
+// where the numbers up to 255 u, the first normal ones among them, are still evenly spaced).
+//
+// A bfloat16 X is staged times 2^110, so that its products with such numbers lie well inside the range of 32 bits, and times
+// 2^106 where it meets a 16 q u; a 32-bit X as three such columns of 8 bits each, which sum up to it exactly.  A binary16 X is
+// staged as it is (a sixteenth of its smallest numbers could not be written) and the products with 16 q u are summed apart.
+// Infinities and NaN, and numbers from 2^18 on in the wide types, make every output of their row infinite or NaN: outputs
+// that are get computed once more as the formula has it.  At the other end the products end at 2^-126.
+//
+// Zero points leave the products:  sum x (q - z) = sum x q - z sum x,  the sums of x by groups taken once per block, in 32
+// bits, where the accumulators start.  That costs the rounding of sum x q, about twice that of the result, and saves a
+// subtraction for two weights.
+//
+// The order of k inside a product is free as long as both operands have it.  A 32-bit word holds k, k + 1, ... k + 7; its
+// AND-OR yields the pairs (k, k + 4), (k + 1, k + 5), ...  So a lane takes whole words of a weight row as they lie, and X is
+// laid out in shared memory, once per block, in the order that matches.
+//
+// A worker of 1, 2, 4 or 8 warps has 32 weight rows at a time; its warps take the steps of 256 k in turn and put their sums
+// together in shared memory.  Workers do not wait for one another (but for clusters, below).  Every warp has a pipeline of
+// its own: its steps (4 KB) come into its stages by TMA, issued by its first lane as soon as a stage has been read, across
+// the ends of a worker's rows too, so that the memory does not wait for sums.  Weight rows that TMA cannot describe (not on
+// 16-byte boundaries) are copied by the lanes in aligned words (cp.async) and shifted into place when they are read.
+//
+// Where there are few weight rows for the SMs, or X is too large for a block's shared memory, the blocks of a cluster share
+// k, and their sums meet through distributed shared memory.
 #pragma once
 
+#include "../../include/cuasr_b200_types.h"
 #include "decode_types.cuh"
 
 namespace cuasr_b200 {
+
+constexpr int kQ4Rows = 32;                   // weight rows of a worker: two tiles of the instruction
+constexpr int kQ4Step = 256;                  // k of a step, two halves of 16 words of a weight row, 4 of them to a lane
+constexpr int kQ4Pitch = kQ4Step / 2 + 4;     // bytes between rows of a stage that the lanes fill: one more aligned word
+template <bool TMA> constexpr int kQ4Stage = kQ4Rows * (TMA ? kQ4Step / 2 : kQ4Pitch);
+constexpr int kQ4MaxStages = 4;
+constexpr int kQ4MaxSlices = 4;               // blocks of a cluster that share k
+template <int NT> constexpr int kQ4Warps = NT == 4 ? 8 : 16;       // the sums of 32 columns leave registers for eight
+constexpr int kQ4SumStride = kQ4Rows + 4;     // floats between columns of a warp's sums: no bank twice
+template <int NT> constexpr int kQ4Buffer = NT * 8 * kQ4SumStride; // floats of a warp's sums
+// X is read eight columns at a time: what lies behind a panel's last word has to be there.
+template <int NT> constexpr int kQ4Overread = NT * 8 * 64;
 
 struct Q4Params {
   const void* X; long long ldx;
@@ -11,46 +54,534 @@ struct Q4Params {
   const void* scales; long long ld_scales;
   const unsigned char* zeros; long long ld_zeros;
   void* Y; long long ldy;
-  int m, n, k, group, groups;
+  int m, n, k, group, groups, group_shift;    // group_shift: log2(group), or -1
+  int type_x, type_y, type_scale;             // cuasr_dtype_t
+  int rows;                                   // rows of X of a pass (blockIdx.y)
+  int units, parts, slices;                   // 32 weight rows each; warps of a worker; blocks that share k
+  int panel_steps;                            // steps whose X fits into shared memory; a multiple of parts if not all
+  int stages, sum_bytes, xsum_bytes;
+  unsigned int* status;
+  bool x_vectors;                             // X can be read 16 bytes at a time
 };
 
-// One warp per weight row and up to four rows of X; the lanes share each group's bytes.
-template <typename TX, typename TY, typename TS>
-__global__ void __launch_bounds__(256) q4_rows_kernel(const Q4Params p) {
-  grid_dependency_wait();
-  grid_dependency_launch();
-  const int lane = threadIdx.x % 32;
-  const long long j = static_cast<long long>(blockIdx.x) * 8 + threadIdx.x / 32;
-  const int r0 = blockIdx.y * 4;
-  if (j >= p.n) return;
-  const unsigned char* w = p.W + j * p.ldw;
-  const TX* x = static_cast<const TX*>(p.X) + r0 * p.ldx;
-  float acc[4] = {};
-  for (int g = 0; g < p.groups; ++g) {
-    const float scale = to_float(static_cast<const TS*>(p.scales)[j * p.ld_scales + g]);
-    const int zero = p.zeros == nullptr ? 8 : p.zeros[j * p.ld_zeros + g] & 15;
-    const int k_end = min(p.k, (g + 1) * p.group);
-    float part[4] = {};
-    for (int k = g * p.group + 2 * lane; k < k_end; k += 64) {
-      const int byte = w[k / 2];
-      const float lo = static_cast<float>((byte & 15) - zero), hi = static_cast<float>((byte >> 4) - zero);
+__device__ __forceinline__ float load_real(const void* base, long long at, int type) {
+  return type == CUASR_F32 ? static_cast<const float*>(base)[at]
+         : type == CUASR_F16 ? to_float(static_cast<const __half*>(base)[at]) : to_float(static_cast<const __nv_bfloat16*>(base)[at]);
+}
+__device__ __forceinline__ void store_real(void* base, long long at, int type, float v) {
+  if (type == CUASR_F32) static_cast<float*>(base)[at] = v;
+  else if (type == CUASR_F16) static_cast<__half*>(base)[at] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(v);
+}
+
+// d = c + a b of a 16 x 16 and a 16 x 8 tile.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+// The four pairs (k, k + 4) ... (k + 3, k + 7) of a word, the second and the fourth times 16.
+__device__ __forceinline__ void pairs_of(uint32_t w, uint32_t (&out)[4]) {
+  out[0] = w & 0x000F000Fu;
+  out[1] = w & 0x00F000F0u;
+  const uint32_t upper = w >> 8;
+  out[2] = upper & 0x000F000Fu;
+  out[3] = upper & 0x00F000F0u;
+}
+
+// Memory word of half a step that word i of lane t of a quad is.  A group's products are summed apart, so the four lanes of an
+// instruction share a group: LW words in a row go to a lane, 4 where groups are whole steps, 2 for groups of 64, 1 for 32.
+template <int LW>
+__device__ __forceinline__ int word_index(int i, int t) {
+  return LW == 4 ? t * 4 + i : LW == 2 ? (i / 2) * 8 + t * 2 + i % 2 : i * 4 + t;
+}
+
+// Half a stage holds its rows 64 bytes apart, their four 16-byte chunks exchanged as TMA's 64-byte swizzle does it: the
+// words that eight rows and four lanes read at a time lie in different banks.
+__device__ __forceinline__ int chunk_at(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 1 & 3)) << 4); }
+
+// Words 0 .. 3 of lane (g, t) from row g + 8 j of half a stage.
+template <int LW>
+__device__ __forceinline__ void read_words(uint32_t (&w)[4], const unsigned char* half, int j, int g, int t) {
+  const unsigned char* row = half + j * 512;
+  if constexpr (LW == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + chunk_at(g, t));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (LW == 2) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (r0 + r >= p.m) break;
-        part[r] = fmaf(lo, to_float(x[r * p.ldx + k]), part[r]);
-        if (k + 1 < k_end) part[r] = fmaf(hi, to_float(x[r * p.ldx + k + 1]), part[r]);
-      }
+    for (int i = 0; i < 4; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(row + chunk_at(g, i + t / 2) + t % 2 * 8);
+      w[i] = v.x; w[i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(row + chunk_at(g, i) + t * 4);
+  }
+}
+// ... from a stage that the lanes filled, whose row j starts `shift` / 8 bytes into its first word.
+template <int LW>
+__device__ __forceinline__ void read_words_shifted(uint32_t (&w)[4], const unsigned char* half, int j, int g, int t, unsigned int shift) {
+  const uint32_t* row = reinterpret_cast<const uint32_t*>(half + (j * 8 + g) * kQ4Pitch);
+#pragma unroll
+  for (int i = 0; i < 4; i += LW) {
+    const int first = word_index<LW>(i, t);
+    uint32_t v = row[first];
+#pragma unroll
+    for (int e = 0; e < LW; ++e) {
+      const uint32_t more = row[first + e + 1];
+      w[i + e] = __funnelshift_r(v, more, shift);
+      v = more;
+    }
+  }
+}
+
+// The lanes' way to copy a step: lane l has word l of every row, lane r also the last word (of 33) of row r.  Words reach over the
+// ends of a row into its neighbours'; those that would reach outside of [W, last) are put together from its bytes.
+__device__ __forceinline__ void copy_word(const Q4Params& p, unsigned char* stage, long long row, int step, int r, int word, int row_bytes,
+                                          const unsigned char* last) {
+  unsigned char* to = stage + r * kQ4Pitch + word * 4;
+  const unsigned char* q = p.W + row * p.ldw + static_cast<long long>(step) * (kQ4Step / 2);
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(q) & 3);
+  const int at = step * (kQ4Step / 2) + word * 4 - off;         // of the row
+  if (row >= p.n || at >= row_bytes) {
+    *reinterpret_cast<uint32_t*>(to) = 0;
+    return;
+  }
+  const unsigned char* a = q - off + word * 4;
+  if (a >= p.W && a + 4 <= last) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(a) : "memory");
+  } else {
+    uint32_t v = 0;
+    for (int b = 0; b < 4; ++b)
+      if (a + b >= p.W && a + b < last) v |= static_cast<uint32_t>(a[b]) << (8 * b);
+    *reinterpret_cast<uint32_t*>(to) = v;
+  }
+}
+__device__ __forceinline__ void copy_step(const Q4Params& p, unsigned char* stage, long long first_row, int step, int lane, int row_bytes,
+                                          const unsigned char* last) {
+#pragma unroll 4
+  for (int r = 0; r < kQ4Rows; ++r) copy_word(p, stage, first_row + r, step, r, lane, row_bytes, last);
+  copy_word(p, stage, first_row + lane, step, lane, 32, row_bytes, last);
+}
+
+// Eight values of a row of X from k on, zeros from p.k on: E = uint32_t for 32-bit rows, unsigned short for 16-bit ones.
+template <typename E>
+__device__ __forceinline__ void load_x8(const Q4Params& p, long long row, int k, uint32_t (&x)[2 * sizeof(E)]) {
+  const E* at = static_cast<const E*>(p.X) + row * p.ldx + k;
+  if (p.x_vectors && k + 8 <= p.k) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(E)) / 2; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(at)[i];
+      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    }
+  } else {
+    uint32_t e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = k + i < p.k ? at[i] : 0u;
+#pragma unroll
+    for (int i = 0; i < 2 * static_cast<int>(sizeof(E)); ++i) x[i] = sizeof(E) == 4 ? e[i] : e[2 * i % 8] | e[(2 * i + 1) % 8] << 16;
+  }
+}
+
+// What the products are multiplied by in the end.
+template <bool BF16> constexpr float kQ4Back = BF16 ? 8388608.0f : 16777216.0f;       // 2^23, 2^24
+
+// Lays out X for steps [begin, end): 16 bytes for each (half a step, word of a lane, column, lane of a quad), and -z times the
+// sums by groups (z = 8, or 1 where zero points are given).  Columns are the rows of X; a 32-bit row is three.
+// Not inlined: it runs once a panel, and its registers are not to crowd out those of the products.
+template <bool BF16, typename E, int LW, int THREADS>
+__device__ __noinline__ void stage_x(const Q4Params& p, uint4* xs, float* xsums, int r0, int rows, int columns, int pitch, int begin, int end) {
+  constexpr int kBatch = 8 / sizeof(E);                       // loads of as many items are in flight
+  constexpr int kLanes = LW * 4;                              // words of a group
+  constexpr int kAtOnce = THREADS / 32;
+  const float z = (p.zeros == nullptr ? -8.0f : -1.0f) / kQ4Back<BF16>;
+  const int lane = threadIdx.x % 32, steps = end - begin, in_half = lane % 16;
+  const int i = LW == 4 ? in_half % 4 : LW == 2 ? in_half / 8 * 2 + in_half % 2 : in_half / 4;
+  const int t = LW == 4 ? in_half / 4 : LW == 2 ? in_half / 2 % 4 : in_half % 4;
+  uint4* const xs_lane = xs + (lane / 16 * 4 + i) * columns * 4 + t;
+  float* const sums_lane = xsums + (lane / 16 * (4 / LW) + in_half / kLanes) * pitch;
+  // a warp takes a step of a row (32 words) at a time: row r, step s behind `begin`
+  int r = threadIdx.x / 32 / steps, s = threadIdx.x / 32 % steps;
+  auto next = [&](int& row, int& step) {
+    step += kAtOnce;
+    while (step >= steps) { step -= steps; ++row; }
+  };
+  while (r < rows) {
+    uint32_t bits[kBatch][2 * sizeof(E)];
+    int row = r, step = s;
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      if (row < rows) load_x8<E>(p, r0 + row, (begin + step) * kQ4Step + lane * 8, bits[q]);
+      next(row, step);
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc[r] = fmaf(scale, part[r], acc[r]);
-  }
+    for (int q = 0; q < kBatch; ++q) {
+      if (r >= rows) break;
+      uint4* to = xs_lane + (s * 8 * columns + r) * 4;
+      float x[8];
+      if constexpr (sizeof(E) == 4) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    float s = acc[r];
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(bits[q][e]);
+      } else {
+        const uint4 v = make_uint4(bits[q][0], bits[q][1], bits[q][2], bits[q][3]);
+        if constexpr (BF16) unpack16(v, x, __nv_bfloat16());
+        else unpack16(v, x, __half());
+      }
+      float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (lane == 0 && r0 + r < p.m) static_cast<TY*>(p.Y)[(r0 + r) * p.ldy + j] = from_float<TY>(s);
+      for (int o = kLanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      if (in_half % kLanes == 0) {
+        float* to_sum = sums_lane + s * (8 / LW) * pitch + r;
+        *to_sum = z * sum;
+        if constexpr (sizeof(E) == 4) to_sum[rows] = to_sum[2 * rows] = 0.0f;       // the whole sum goes with the first column
+      }
+      constexpr float up = 1.298074214633707e33f, up16 = up / 16;                   // 2^110
+      if constexpr (sizeof(E) == 2) {
+        const uint32_t(&v)[4] = bits[q];
+        uint4 pairs = make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410),
+                                 __byte_perm(v[1], v[3], 0x7632));
+        if constexpr (BF16) {
+          auto times = [](uint32_t a, float by) {
+            const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), __float2bfloat162_rn(by));
+            return *reinterpret_cast<const uint32_t*>(&h);
+          };
+          *to = make_uint4(times(pairs.x, up), times(pairs.y, up16), times(pairs.z, up), times(pairs.w, up16));
+        } else {
+          *to = make_uint4(pairs.x, pairs.z, pairs.y, pairs.w);       // the pairs that meet q first, then those that meet 16 q
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= e % 2 == 0 ? up : up16;
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            h[e] = __float_as_uint(x[e]) >> 16;                       // the upper half: a bfloat16, rounded towards zero
+            x[e] -= __uint_as_float(h[e] << 16);
+          }
+          to[part * rows * 4] = make_uint4(h[0] | h[4] << 16, h[1] | h[5] << 16, h[2] | h[6] << 16, h[3] | h[7] << 16);
+        }
+      }
+      next(r, s);
+    }
   }
+}
+
+// Row r of X times weight row j as the formula has it.
+static __device__ __noinline__ float plain_dot(const Q4Params& p, int r, long long j) {
+  float sum = 0.0f;
+  for (int group = 0; group < p.groups; ++group) {
+    const int zero = p.zeros == nullptr ? 8 : p.zeros[j * p.ld_zeros + group] & 15;
+    const long long stop = min(static_cast<long long>(p.k), (group + 1LL) * p.group);
+    float part = 0.0f;
+    for (long long k = static_cast<long long>(group) * p.group; k < stop; ++k) {
+      const int q = p.W[j * p.ldw + k / 2] >> (k % 2 * 4) & 15;
+      part = fmaf(static_cast<float>(q - zero), load_real(p.X, r * p.ldx + k, p.type_x), part);
+    }
+    sum = fmaf(load_real(p.scales, j * p.ld_scales + group, p.type_scale), part, sum);
+  }
+  return sum;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_cluster(const float* mine, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void worker_barrier(int worker, int warps) {
+  asm volatile("bar.sync %0, %1;" ::"r"(worker + 1), "r"(warps * 32) : "memory");
+}
+
+// NT tiles of eight columns of X.
+template <bool BF16, int NT, int LW, bool TMA, bool ZEROS>
+__global__ void __launch_bounds__(32 * kQ4Warps<NT>, 1)
+q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Params p) {
+  extern __shared__ __align__(1024) unsigned char q4_smem[];
+  constexpr int kThreads = 32 * kQ4Warps<NT>, RT = kQ4Rows / 16;
+  __shared__ uint64_t full[kQ4Warps<NT>][kQ4MaxStages];
+  __shared__ unsigned int abandoned;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  const int parts = p.parts, part_of = warp % parts, local = warp / parts, workers_here = kQ4Warps<NT> / parts;
+  unsigned char* stages = q4_smem + warp * p.stages * kQ4Stage<TMA>;
+  float* all_sums = reinterpret_cast<float*>(q4_smem + kQ4Warps<NT> * p.stages * kQ4Stage<TMA>);
+  const int buffers = max(parts - 1, 1);                   // of a worker
+  float* sums = all_sums + local * buffers * kQ4Buffer<NT>;
+  float* xsums = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(all_sums) + p.sum_bytes);
+  uint4* xs = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(xsums) + p.xsum_bytes);
+  const int slice = p.slices > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int r0 = blockIdx.y * p.rows, rows = min(p.rows, p.m - r0);
+  const int columns = p.type_x == CUASR_F32 ? 3 * rows : rows;
+  const int pitch = (columns + 1) / 2 * 2;       // of xsums
+  const int all_steps = (p.k + kQ4Step - 1) / kQ4Step;
+  const int begin = static_cast<int>(static_cast<long long>(all_steps) * slice / p.slices);
+  const int end = static_cast<int>(static_cast<long long>(all_steps) * (slice + 1) / p.slices);
+  const bool one_panel = end - begin <= p.panel_steps;
+  const int worker = static_cast<int>(blockIdx.x) / p.slices * workers_here + local, workers = static_cast<int>(gridDim.x) / p.slices * workers_here;
+  const int rounds = (p.units + workers - 1) / workers;
+
+  if constexpr (TMA) {
+    if (lane == 0) {
+      for (int s = 0; s < p.stages; ++s) mbar_init(&full[warp][s], 1);
+      fence_barrier_init();
+      fence_proxy_async();
+    }
+  }
+  if (tid == 0) abandoned = 0;
+  __syncthreads();
+  grid_dependency_wait();
+  grid_dependency_launch();
+
+  // what comes next into the pipeline: step `ahead` of unit `ahead_unit`, into stage `ahead_stage`
+  int ahead_unit = begin + part_of < end ? worker : p.units, ahead = begin + part_of, ahead_stage = 0;
+  const int row_bytes = (p.k + 1) / 2;
+  auto copy_ahead = [&] {           // TMA: lane 0 alone
+    if (ahead_unit < p.units) {
+      unsigned char* to = stages + ahead_stage * kQ4Stage<TMA>;
+      if constexpr (TMA) {
+        uint64_t* bar = &full[warp][ahead_stage];
+        const int y = ahead_unit * kQ4Rows, x = ahead * (kQ4Step / 2);
+        mbar_arrive_expect_tx(bar, kQ4Stage<TMA>);
+        tma_load_2d(to, &map, bar, x, y);
+        tma_load_2d(to + kQ4Stage<TMA> / 2, &map, bar, x + kQ4Step / 4, y);
+      } else {
+        copy_step(p, to, static_cast<long long>(ahead_unit) * kQ4Rows, ahead, lane, row_bytes, p.W + (p.n - 1) * p.ldw + row_bytes);
+      }
+      ahead += parts;
+      if (ahead >= end) { ahead = begin + part_of; ahead_unit += workers; }
+      if (++ahead_stage == p.stages) ahead_stage = 0;
+    }
+    if constexpr (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (!TMA || lane == 0)
+    for (int s = 0; s < (TMA ? p.stages : p.stages - 1); ++s) copy_ahead();
+
+  // Scales and zero points of a step, loaded one step ahead, for both its halves.  Where half a step has one group, lane
+  // (g, t) has those of row t * 8 + g; else those of its t-th group for rows g, 8 + g, ...
+  constexpr int kMine = LW == 4 ? 1 : 4;
+  uint32_t next_scale[2][kMine], next_zero[2][kMine];
+  const int scale_shift = p.type_scale == CUASR_BF16 ? 16 : 0;
+  auto load_scales = [&](int unit, int step) {
+    if (unit >= p.units || step >= end) return;
+    // the bits are converted where they are used, so that nothing waits here
+    int group[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int k = step * kQ4Step + u * (kQ4Step / 2) + (LW == 4 ? 0 : LW == 2 ? t / 2 * 64 : t * 32);
+      group[u] = min(p.group_shift >= 0 ? k >> p.group_shift : k / p.group, p.groups - 1);
+    }
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const long long row = min(unit * kQ4Rows + (LW == 4 ? t : j) * 8 + g, p.n - 1);      // rows behind the last get the last one's
+      const long long at = row * p.ld_scales;
+      if (p.type_scale == CUASR_F32) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) next_scale[u][j] = __ldg(static_cast<const unsigned int*>(p.scales) + at + group[u]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) next_scale[u][j] = __ldg(static_cast<const unsigned short*>(p.scales) + at + group[u]);
+      }
+      if constexpr (ZEROS) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) next_zero[u][j] = __ldg(p.zeros + row * p.ld_zeros + group[u]);
+      }
+    }
+  };
+  load_scales(worker, begin + part_of);
+
+  int stage = 0;
+  uint32_t parity = 0;
+  for (int round = 0; round < rounds; ++round) {
+    const int unit = worker + round * workers;
+    const bool mine = unit < p.units;
+    // rows that do not start on a word: how far into it, the same for every step
+    unsigned int shift[TMA ? 1 : 2 * RT];
+    if constexpr (!TMA) {
+#pragma unroll
+      for (int j = 0; j < 2 * RT; ++j)
+        shift[j] = static_cast<unsigned int>((reinterpret_cast<uintptr_t>(p.W) + (static_cast<long long>(unit) * kQ4Rows + j * 8 + g) * p.ldw) & 3) * 8;
+    }
+    float acc[RT][NT][4] = {};
+    for (int panel = begin; panel < end; panel += p.panel_steps) {
+      const int panel_end = min(end, panel + p.panel_steps);
+      if (!one_panel || round == 0) {
+        if (!one_panel) __syncthreads();       // the panel before has been read
+        if constexpr (BF16) {
+          if (p.type_x == CUASR_F32) stage_x<true, uint32_t, LW, kThreads>(p, xs, xsums, r0, rows, columns, pitch, panel, panel_end);
+          else stage_x<true, unsigned short, LW, kThreads>(p, xs, xsums, r0, rows, columns, pitch, panel, panel_end);
+        } else {
+          stage_x<false, unsigned short, LW, kThreads>(p, xs, xsums, r0, rows, columns, pitch, panel, panel_end);
+        }
+        __syncthreads();
+      }
+      if (!mine) continue;
+      for (int step = panel + part_of; step < panel_end; step += parts) {
+        float scale[2][kMine], zero[2][kMine];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) {
+            scale[u][j] = p.type_scale == CUASR_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(next_scale[u][j])))
+                                                    : __uint_as_float(next_scale[u][j] << scale_shift);
+            if constexpr (ZEROS) zero[u][j] = static_cast<float>(next_zero[u][j] & 15u);
+          }
+        if (step + parts < end) load_scales(unit, step + parts);
+        else load_scales(unit + workers, begin + part_of);
+        if constexpr (TMA) {
+          mbar_wait_or_abandon(&full[warp][stage], parity, p.status, kDeviceTimeoutFull, &abandoned);
+        } else {
+          copy_ahead();                // into the stage that was read last
+          if (p.stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+          else if (p.stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+          else asm volatile("cp.async.wait_group 3;" ::: "memory");
+          __syncwarp();
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const unsigned char* words = stages + stage * kQ4Stage<TMA> + (TMA ? u * kQ4Stage<TMA> / 2 : u * kQ4Step / 4);
+          const uint4* x = xs + (((step - panel) * 2 + u) * 16 * columns + lane);
+          uint32_t w[2 * RT][4];
+#pragma unroll
+          for (int j = 0; j < 2 * RT; ++j) {
+            if constexpr (TMA) read_words<LW>(w[j], words, j, g, t);
+            else read_words_shifted<LW>(w[j], words, j, g, t, shift[j]);
+          }
+          const float* xsum = xsums + ((step - panel) * 2 + u) * (4 / LW) * pitch + t * 2;
+          constexpr int kSums = BF16 ? 1 : 2;            // products with q, and with 16 q
+          float part[kSums][RT][NT][4], f[2 * RT];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float2 start[NT];
+            float z[2 * RT];
+            if (i % LW == 0) {
+#pragma unroll
+              for (int j = 0; j < 2 * RT; ++j) {
+                const int from = (lane & ~3) + (LW == 4 ? j : LW == 2 ? i / 2 * 2 : i), of = LW == 4 ? 0 : j;
+                f[j] = __shfl_sync(0xFFFFFFFFu, scale[u][of], from);
+                if constexpr (ZEROS) z[j] = __shfl_sync(0xFFFFFFFFu, zero[u][of], from);
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) start[nt] = *reinterpret_cast<const float2*>(xsum + i / LW * pitch + nt * 8);
+            }
+            uint4 b[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              b[nt] = x[(i * columns + nt * 8) * 4];        // behind the last column: whatever follows, in columns nobody reads
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              uint32_t lo[4], hi[4];
+              pairs_of(w[2 * rt][i], lo);
+              pairs_of(w[2 * rt + 1][i], hi);
+              const uint32_t a0[4] = {lo[0], hi[0], lo[BF16 ? 1 : 2], hi[BF16 ? 1 : 2]}, a1[4] = {lo[BF16 ? 2 : 1], hi[BF16 ? 2 : 1], lo[3], hi[3]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float(&d)[4] = part[0][rt][nt];
+                float(&d16)[4] = part[kSums - 1][rt][nt];
+                if (i % LW == 0) {
+                  const float2 s = start[nt];
+                  if constexpr (ZEROS) mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, z[2 * rt] * s.x, z[2 * rt] * s.y, z[2 * rt + 1] * s.x, z[2 * rt + 1] * s.y);
+                  else mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, s.x, s.y, s.x, s.y);
+                } else {
+                  mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, d[0], d[1], d[2], d[3]);
+                }
+                if (!BF16 && i % LW == 0) mma_16816<BF16>(d16, a1, b[nt].z, b[nt].w, 0.0f, 0.0f, 0.0f, 0.0f);
+                else mma_16816<BF16>(d16, a1, b[nt].z, b[nt].w, d16[0], d16[1], d16[2], d16[3]);
+                if (i % LW == LW - 1) {
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) acc[rt][nt][c] = fmaf(f[2 * rt + c / 2], BF16 ? d[c] : fmaf(d16[c], 0.0625f, d[c]), acc[rt][nt][c]);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();                  // the stage has been read
+        if constexpr (TMA) {
+          if (lane == 0) copy_ahead();
+        }
+        if (++stage == p.stages) { stage = 0; parity ^= 1; }
+      }
+    }
+
+    // All but one warp of the worker put their sums down; that one, another every time, adds them to its own.
+    const int first_row = unit * kQ4Rows, last_row = min(kQ4Rows, p.n - first_row) - 1;
+    auto each_sum = [&](auto&& f) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) f((nt * 8 + t * 2 + c % 2) * kQ4SumStride + rt * 16 + c / 2 * 8 + g, acc[rt][nt][c]);
+    };
+    const int adder = round % parts;
+    if (mine) {
+      if (parts > 1) {
+        worker_barrier(local, parts);      // the sums before have been read
+        if (part_of != adder) {
+          float* to = sums + (part_of < adder ? part_of : part_of - 1) * kQ4Buffer<NT>;
+          each_sum([&](int at, float v) { to[at] = v; });
+        }
+        worker_barrier(local, parts);
+      }
+      if (part_of == adder) {
+        for (int v = 0; v < parts - 1; ++v) each_sum([&](int at, float& a) { a += sums[v * kQ4Buffer<NT> + at]; });
+        each_sum([&](int at, float v) { sums[at] = v; });
+      }
+      if (p.slices == 1) {
+        // the rows of X are shared out among the warps
+        if (parts > 1) worker_barrier(local, parts);
+        else __syncwarp();
+        if (lane <= last_row)
+          for (int r = part_of; r < rows; r += parts) {
+            float s = sums[r * kQ4SumStride + lane];
+            if (columns != rows) s += sums[(r + rows) * kQ4SumStride + lane] + sums[(r + 2 * rows) * kQ4SumStride + lane];
+            s *= kQ4Back<BF16>;
+            if (!isfinite(s)) s = plain_dot(p, r0 + r, first_row + lane);
+            store_real(p.Y, (r0 + r) * p.ldy + first_row + lane, p.type_y, s);
+          }
+        if (parts == 1) __syncwarp();
+      }
+    }
+    if (p.slices > 1) {
+      cluster_barrier();
+      // this block's share of the outputs of its own units, from the sums of all blocks
+      const int outputs = workers_here * rows * kQ4Rows;
+      for (int at = slice * kThreads + tid; at < outputs; at += p.slices * kThreads) {
+        const int j = at % kQ4Rows, r = at / kQ4Rows % rows, l = at / kQ4Rows / rows;
+        const long long row = (static_cast<long long>(worker - local + l) + static_cast<long long>(round) * workers) * kQ4Rows + j;
+        if (row >= p.n) continue;
+        const float* from = all_sums + l * buffers * kQ4Buffer<NT> + r * kQ4SumStride + j;
+        float s = 0.0f;
+        for (int v = 0; v < p.slices; ++v) {
+          float rest = 0.0f;
+          if (columns != rows) rest = load_cluster(from + rows * kQ4SumStride, v) + load_cluster(from + 2 * rows * kQ4SumStride, v);
+          s += load_cluster(from, v) + rest;
+        }
+        s *= kQ4Back<BF16>;
+        if (!isfinite(s)) s = plain_dot(p, r0 + r, row);
+        store_real(p.Y, (r0 + r) * p.ldy + row, p.type_y, s);
+      }
+      cluster_barrier();                     // no block writes its sums before all have read them
+    }
+  }
+  if constexpr (!TMA) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 }  // namespace cuasr_b200
