@@ -3,19 +3,29 @@
 //   value(b, v) = (score[b] - log sum_u exp(logit[b, u])) + logit[b, v]
 //
 // Within a prefix the values order as its logits do, so one pass over the logits finds both the sum and the prefix's own
-// `keep` best; the searches' best are then chosen among those.
+// `keep` best; the searches' best are then chosen among those.  The floor is the logits' bytes at the memory's rate, which
+// leaves about eleven instructions of a lane for a 16-bit logit and twice as many for a 32-bit one; so exponentials are worked out in pairs, and a logit is otherwise only part of a maximum, which is
+// compared with a bound that nearly all threads stay below.  The bound comes from the threads' own maxima and is taken
+// again after 1, 2, 4, ... tiles; a row of 16 tiles then has about seven candidates for each that is kept, which every warp
+// collects by itself and which are sorted once, at the row's end.
 #pragma once
 
 #include "decode_types.cuh"
 
 namespace cuasr_b200 {
 
-constexpr int kBeamThreads = 256;
-constexpr int kBeamItems = 16;                                  // logits of a thread per tile
-constexpr int kBeamTile = kBeamThreads * kBeamItems;
-constexpr int kBeamList = 1024;                                 // candidates kept between tiles before they are thinned out
-constexpr int kBeamMergeTile = 4 * kBeamThreads;
-constexpr int kBeamMergeList = 512;
+constexpr int kBeamThreads = 128;
+constexpr int kBeamVectors = 4;                                 // 16-byte vectors of a thread per tile
+constexpr int kBeamTileBytes = kBeamThreads * kBeamVectors * 16;
+constexpr int kBeamStages = 3;
+constexpr int kBeamBlocks = 7;                                  // of an SM
+constexpr int kBeamWarps = kBeamThreads / 32;
+constexpr int kBeamSegment = 128;                               // candidates that a warp can hold after a tile ...
+constexpr int kBeamStride = kBeamSegment + 8;                   // ... and the few logits behind the last
+constexpr int kBeamCapacity = kBeamWarps * kBeamStride;
+constexpr int kBeamRanked = kBeamThreads;                                // up to so many are sorted by comparing all with all
+constexpr int kMergeThreads = 256;
+constexpr int kBeamMergeMost = 8192;                            // candidates that are merged in shared memory
 
 struct BeamParams {
   const void* logits; long long batch_stride, beam_stride;
@@ -28,6 +38,8 @@ struct BeamParams {
   double* part_sum;                // [batch * beams * parts]: sum of exp(logit - part_max)
   float* part_max;
   int batch, beams, vocab, keep, parts, end_token, normalise;
+  int chunk;                       // vectors of a part
+  unsigned int* status;
 };
 
 // Whole numbers that order as (logit, lower token first); 0 is no candidate.
@@ -51,6 +63,31 @@ __device__ __forceinline__ float exp_of(float d) {
   return r;
 }
 
+// ... of a pair.
+__device__ __forceinline__ uint64_t exp_of_pair(uint64_t d) {
+  const uint64_t y = fma2(d, pack2(1.44269502162933349609375f, 1.44269502162933349609375f),
+                          mul2(d, pack2(1.92596299112661746887e-8f, 1.92596299112661746887e-8f)));
+  float a, b;
+  unpack2(y, a, b);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return pack2(a, b);
+}
+// The largest of the elements of 16 bytes; NaN only if all are.
+__device__ __forceinline__ float largest(const uint4& v, float) {
+  return fmaxf(max3(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z)), __uint_as_float(v.w));
+}
+__device__ __forceinline__ float largest(const uint4& v, __half) {
+  auto h = [](const uint32_t& a) { return *reinterpret_cast<const __half2*>(&a); };
+  const float2 f = __half22float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
+  return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ float largest(const uint4& v, __nv_bfloat16) {
+  auto h = [](const uint32_t& a) { return *reinterpret_cast<const __nv_bfloat162*>(&a); };
+  const float2 f = __bfloat1622float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
+  return fmaxf(f.x, f.y);
+}
+
 // The largest float below x (x finite or +infinity; -infinity stays).
 __device__ __forceinline__ float float_below(float x) {
   if (x == 0.0f) return -__uint_as_float(1u);
@@ -59,295 +96,534 @@ __device__ __forceinline__ float float_below(float x) {
   return __uint_as_float(bits >> 31 ? bits + 1 : bits - 1);
 }
 
-// A list of candidate keys in shared memory that `keep` survivors are chosen from.
-struct BeamList {
-  unsigned long long* keys;    // kBeamList + kBeamTile
-  int* count;
-};
-
-// The keep-th largest of n distinct keys, found bit by bit.  All threads call it.
-__device__ __forceinline__ unsigned long long kth_key(const unsigned long long* keys, int n, int keep, int* counter) {
-  unsigned long long found = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const unsigned long long probe = found | 1ull << bit;
-    int c = 0;
-    for (int i = threadIdx.x; i < n; i += kBeamThreads) c += keys[i] >= probe;
-    c = __reduce_add_sync(0xFFFFFFFFu, c);
-    if (threadIdx.x == 0) *counter = 0;
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) atomicAdd(counter, c);
-    __syncthreads();
-    if (*counter >= keep) found = probe;
-    __syncthreads();
+// The j-th largest of the lanes' values (j >= 1); equal ones count apart.
+__device__ __forceinline__ float warp_jth(float x, int j) {
+  const unsigned int bits = __float_as_uint(x + 0.0f);
+  unsigned int up = bits >> 31 ? ~bits : bits | 0x80000000u, top = 0;
+  for (; j > 0; --j) {
+    top = __reduce_max_sync(0xFFFFFFFFu, up);
+    const unsigned int who = __ballot_sync(0xFFFFFFFFu, up == top);
+    if ((threadIdx.x & 31) == __ffs(who) - 1) up = 0;
   }
-  return found;
+  return top == 0 ? -INFINITY : __uint_as_float(top >> 31 ? top & 0x7FFFFFFFu : ~top);
 }
 
-// Leaves the `keep` largest of the list at its front, in no order; returns the smallest of them.
-__device__ __forceinline__ unsigned long long thin_out(const BeamList& list, int keep, int* counter) {
+// A lower bound for the keep-th largest of the threads' values, where the first `warps` of the block have some: each has at
+// least keep / warps at or above its own, and the smallest of these bounds is taken.  All threads call it.
+__device__ __forceinline__ float block_bound(float x, int keep, int warps, float* scratch) {
+  const float mine = warp_jth(x, (keep + warps - 1) / warps);
+  if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = mine;
   __syncthreads();
-  const int n = *list.count;
-  const unsigned long long least = kth_key(list.keys, n, keep, counter);
-  constexpr int kMost = (kBeamList + kBeamTile + kBeamThreads - 1) / kBeamThreads;
-  unsigned long long mine[kMost];
+  float bound = scratch[0];
 #pragma unroll
-  for (int i = 0; i < kMost; ++i) {
-    const int at = i * kBeamThreads + threadIdx.x;
-    mine[i] = at < n ? list.keys[at] : 0;
+  for (int w = 1; w < kBeamWarps; ++w) bound = w < warps ? fminf(bound, scratch[w]) : bound;
+  return bound;
+}
+
+// Number of threads' counts, summed over the block.
+__device__ __forceinline__ int block_sum(int c, int* counter) {
+  c = __reduce_add_sync(0xFFFFFFFFu, c);
+  if (threadIdx.x == 0) *counter = 0;
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) atomicAdd(counter, c);
+  __syncthreads();
+  c = *counter;
+  __syncthreads();
+  return c;
+}
+
+// A tile with more candidates than a warp holds: the `keep` largest among the keys from before the tile (tokens below the
+// tile's; segment w of `keys` has counts[w]) and the tile's logits, which are read once more.  They are dealt out to the
+// segments in turn; returns the smallest.  The tile: vectors [base, end) of xv, the first logit of which is token `head`.
+template <typename T>
+__device__ __noinline__ unsigned long long thin_out_tile(unsigned long long* keys, const int* counts, int* counter, const uint4* xv, int base, int end,
+                                                         int head, int keep) {
+  constexpr int V = Vec16<T>::count, kScan = kBeamWarps * kBeamSegment / kBeamThreads;
+  const int tid = threadIdx.x, first = head + base * V;
+  unsigned long long before[kScan], least = 0;
+#pragma unroll
+  for (int i = 0; i < kScan; ++i) {
+    const int at = i * kBeamThreads + tid;
+    before[i] = at % kBeamSegment < counts[at / kBeamSegment] ? keys[at / kBeamSegment * kBeamStride + at % kBeamSegment] : 0;
+    if (beam_key_token(before[i]) >= first) before[i] = 0;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) *list.count = 0;
-  __syncthreads();
+  // the logits are read anew in every pass: this is rare, and its registers would be the kernel's
+  auto each = [&](auto&& f) {
+#pragma unroll 1
+    for (int u = 0; u < kBeamVectors; ++u) {
+      const int at = base + u * kBeamThreads + tid;
+      if (at >= end) break;
+      float x[V];
+      unpack16(xv[at], x, T());
 #pragma unroll
-  for (int i = 0; i < kMost; ++i)
-    if (mine[i] != 0 && mine[i] >= least) list.keys[atomicAdd(list.count, 1)] = mine[i];
+      for (int e = 0; e < V; ++e) f(x[e] > -INFINITY ? beam_key(x[e], head + at * V + e) : 0ull);
+    }
+  };
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long probe = least | 1ull << bit;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kScan; ++i) c += before[i] >= probe;
+    each([&](unsigned long long key) { c += key >= probe; });
+    if (block_sum(c, counter) >= keep) least = probe;
+  }
+  if (tid == 0) *counter = 0;
+  __syncthreads();
+  auto add = [&](unsigned long long key) {
+    if (key == 0 || key < least) return;
+    const int at = atomicAdd(counter, 1);
+    keys[at % kBeamWarps * kBeamStride + at / kBeamWarps] = key;
+  };
+#pragma unroll
+  for (int i = 0; i < kScan; ++i) add(before[i]);
+  each(add);
   __syncthreads();
   return least;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const BeamParams p) {
-  extern __shared__ unsigned long long beam_smem[];
-  __shared__ int count, counter;
-  __shared__ float maxima[kBeamThreads];
-  __shared__ double sums[kBeamThreads / 32];
-  __shared__ float limit;
-  constexpr int V = Vec16<T>::count, U = kBeamItems / V;
+// More than kBeamRanked keys: leaves the `keep` largest at the front, in no order.
+__device__ __noinline__ void thin_out(unsigned long long* keys, int n, int keep, int* counter) {
+  constexpr int kMost = (kBeamCapacity + kBeamThreads - 1) / kBeamThreads;
   const int tid = threadIdx.x;
-  const long long row = blockIdx.x / p.parts;
-  const int part = blockIdx.x % p.parts;
-  const int batch = static_cast<int>(row / p.beams), beam = static_cast<int>(row % p.beams);
+  unsigned long long mine[kMost], least = 0;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) mine[i] = i * kBeamThreads + tid < n ? keys[i * kBeamThreads + tid] : 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long probe = least | 1ull << bit;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) c += mine[i] >= probe;
+    if (block_sum(c, counter) >= keep) least = probe;
+  }
+  if (tid == 0) *counter = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMost; ++i)
+    if (mine[i] != 0 && mine[i] >= least) keys[atomicAdd(counter, 1)] = mine[i];
+  __syncthreads();
+}
+
+// A block has part blockIdx.y of row blockIdx.x: of its vectors `chunk`, and the few logits in front with the first part, those behind
+// with the last.
+template <typename T, bool NORMALISE>
+__global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(const BeamParams p) {
+  extern __shared__ __align__(128) uint4 beam_tiles[];            // kBeamStages tiles
+  __shared__ unsigned long long keys[kBeamCapacity];
+  __shared__ uint64_t full[kBeamStages];
+  __shared__ int counter, counts[kBeamWarps];
+  __shared__ float maxima[kBeamWarps];
+  __shared__ double sums[kBeamWarps];
+  __shared__ unsigned int abandoned;
+  constexpr int V = Vec16<T>::count, U = kBeamVectors, kTile = kBeamThreads * U;
+  constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;     // -infinity
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int part = blockIdx.y, batch = static_cast<int>(blockIdx.x) / p.beams, beam = static_cast<int>(blockIdx.x) - batch * p.beams;
+  if (tid == 0) {
+    abandoned = 0;
+    for (int s = 0; s < kBeamStages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+    fence_proxy_async();
+  }
   grid_dependency_wait();
   grid_dependency_launch();
   if (p.finished != nullptr && p.finished[batch * p.ld_finished + beam] != 0) return;
 
-  BeamList list = {beam_smem, &count};
-  if (tid == 0) count = 0;
   const T* x = static_cast<const T*>(p.logits) + batch * p.batch_stride + beam * p.beam_stride;
-  // the row: up to V - 1 logits before the first 16-byte boundary, whole vectors, up to V - 1 logits behind them
-  const int head = min(p.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+  const int head = min(p.vocab, static_cast<int>(-(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (V - 1)));
   const int vectors = (p.vocab - head) / V, tail = p.vocab - head - vectors * V;
-  const int v_begin = static_cast<int>(static_cast<long long>(vectors) * part / p.parts);
-  const int v_end = static_cast<int>(static_cast<long long>(vectors) * (part + 1) / p.parts);
+  const int v_begin = min(part * p.chunk, vectors), v_end = part == p.parts - 1 ? vectors : min(v_begin + p.chunk, vectors);
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-
-  float m = -INFINITY, sum = 0.0f, above = -INFINITY;    // this thread's maximum and sum; candidates are above `above`
-  __syncthreads();
-
-  // the few logits outside of whole vectors, one to a thread: those in front first, those behind last, so that of equal
-  // logits the ones met later always have the higher token
-  auto take_one = [&](int at) {
-    const float value = to_float(x[at]);
-    if (value > above) list.keys[atomicAdd(&count, 1)] = beam_key(value, at);
-    const float m_new = fmaxf(m, value), ref = m_new == -INFINITY ? 0.0f : m_new;
-    sum = fmaf(sum, exp_of(m - ref), exp_of(value - ref));
-    m = m_new;
+  auto copy = [&](int base, int stage) {                 // thread 0
+    if (base >= v_end) return;
+    const uint32_t bytes = static_cast<uint32_t>(min(kTile, v_end - base)) * 16;
+    mbar_arrive_expect_tx(&full[stage], bytes);
+    bulk_load(beam_tiles + stage * kTile, xv + base, bytes, &full[stage]);
   };
-  if (part == 0 && tid < head) take_one(tid);
-  for (int base = v_begin; base < v_end; base += kBeamThreads * U) {
-    float v[U][V];
+  if (tid == 0)
+    for (int s = 0; s < kBeamStages; ++s) copy(v_begin + s * kTile, s);
+
+  float m = -INFINITY, sum = 0.0f;                       // this thread's maximum and sum
+  float above = -INFINITY, floor = -INFINITY;            // candidates are above `above`; of those found, `keep` reach `floor`
+  int held = 0;                                          // candidates of this warp
+  unsigned long long* segment = keys + warp * kBeamStride;
+  __syncthreads();
+  // one logit of each lane (or none: -infinity) goes to the warp's candidates if it is above the bound
+  auto collect = [&](float value, int token, int room) {
+    const bool in = value > above;
+    const unsigned int who = __ballot_sync(0xFFFFFFFFu, in);
+    if (who != 0) {
+      const int at = held + __popc(who & ((1u << lane) - 1));
+      if (in && at < room) segment[at] = beam_key(value, token);
+      held += __popc(who);
+    }
+  };
+  // the few logits outside of whole vectors, one to a lane of the first warp: those in front first, those behind last, so
+  // that of equal logits the ones met later always have the higher token
+  auto take_one = [&](int at, bool mine) {
+    const float value = mine ? to_float(x[at]) : -INFINITY, m_new = fmaxf(m, value);
+    if constexpr (NORMALISE) {
+      const float ref = m_new == -INFINITY ? 0.0f : m_new;
+      sum = fmaf(sum, exp_of(m - ref), exp_of(value - ref));
+    }
+    m = m_new;
+    collect(value, at, kBeamStride);
+  };
+  if (part == 0 && head > 0 && warp == 0) take_one(lane, lane < head);
+  int stage = 0, tile = 0;
+  uint32_t parity = 0;
+  for (int base = v_begin; base < v_end; base += kTile) {
+    mbar_wait_or_abandon(&full[stage], parity, p.status, kDeviceTimeoutFull, &abandoned);
+    uint4* here = beam_tiles + stage * kTile + tid;
+    if (v_end - base < kTile)                            // the last tile: each thread fills up its own places
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (base + u * kBeamThreads + tid >= v_end) here[u * kBeamThreads] = make_uint4(kNone, kNone, kNone, kNone);
+    float tops[U], top = -INFINITY;                      // not NaN
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = base + u * kBeamThreads + tid;
-      if (at < v_end) unpack16(__ldcs(xv + at), v[u], T());
-      else {
+      tops[u] = largest(here[u * kBeamThreads], T());
+      top = fmaxf(top, tops[u]);
+    }
+    const float m_new = fmaxf(m, top);
+    if constexpr (NORMALISE) {
+      const float ref = m_new == -INFINITY ? 0.0f : m_new;
+      const uint64_t minus = pack2(-ref, -ref);
+      uint64_t s[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[u][e] = -INFINITY;
+      for (int u = 0; u < U; ++u) {
+        float v[V];
+        unpack16(here[u * kBeamThreads], v, T());
+#pragma unroll
+        for (int e = 0; e < V; e += 2) s[e / 2 % 2] = add2(s[e / 2 % 2], exp_of_pair(add2(pack2(v[e], v[e + 1]), minus)));
+      }
+      float a, b;
+      unpack2(add2(s[0], s[1]), a, b);
+      sum = fmaf(sum, exp_of(m - ref), a + b);
+    }
+    m = m_new;
+    if ((tile & (tile - 1)) == 0) {
+      const float bound = block_bound(m, p.keep, min((v_end - v_begin + 31) / 32, kBeamWarps), maxima);
+      if (bound > floor) {
+        floor = bound;
+        above = float_below(bound);
       }
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) top = fmaxf(top, v[u][e]);
-    if (p.normalise) {
-      const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.0f : m_new;
-      float s = 0.0f;
+    ++tile;
+    if (__any_sync(0xFFFFFFFFu, top > above)) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
+        if (__any_sync(0xFFFFFFFFu, tops[u] > above)) {
+          float v[V];
+          unpack16(here[u * kBeamThreads], v, T());
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += exp_of(v[u][e] - ref);
-      sum = fmaf(sum, exp_of(m - ref), s);
-      m = m_new;
+          for (int e = 0; e < V; ++e) collect(v[e], head + (base + u * kBeamThreads + tid) * V + e, kBeamSegment);
+        }
     }
-    if (base == v_begin) {
-      // keep threads have a logit at or above the keep-th largest of the threads' maxima
-      maxima[tid] = top;
-      if (tid == 0) limit = -INFINITY;
+    if (__syncthreads_or(held > kBeamSegment)) {
+      // more than the warp holds (many equal logits, or ever larger ones): what follows lies further along the row, and equal
+      // logits there lose
+      if (lane == 0) counts[warp] = min(held, kBeamSegment);
       __syncthreads();
-      int rank = 0;
-#pragma unroll 8
-      for (int i = 0; i < kBeamThreads; ++i) rank += maxima[i] > top || (maxima[i] == top && i < tid);
-      if (rank == p.keep - 1) limit = float_below(top);
-      __syncthreads();
-      above = limit;
+      floor = above = beam_key_logit(thin_out_tile<T>(keys, counts, &counter, xv, base, v_end, head, p.keep));
+      held = (p.keep - warp + kBeamWarps - 1) / kBeamWarps;
     }
-    if (top > above) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (v[u][e] > above)
-            list.keys[atomicAdd(&count, 1)] = beam_key(v[u][e], head + (base + u * kBeamThreads + tid) * V + e);
-    }
-    __syncthreads();
-    if (count > kBeamList) {
-      // what follows lies further along the row: equal logits there lose
-      above = beam_key_logit(thin_out(list, p.keep, &counter));
-    }
-    __syncthreads();
+    // all have read the stage: the barrier above
+    if (tid == 0) copy(base + kBeamStages * kTile, stage);
+    if (++stage == kBeamStages) { stage = 0; parity ^= 1; }
   }
-  if (part == p.parts - 1 && tid < tail) take_one(p.vocab - tail + tid);
-  __syncthreads();
-  if (count > kBeamMergeList) thin_out(list, p.keep, &counter);
-  __syncthreads();
-  const int n = count;
-  unsigned long long* out = p.part_keys + static_cast<long long>(blockIdx.x) * p.keep;
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const unsigned long long key = list.keys[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += list.keys[j] > key;
-    if (rank < p.keep) out[rank] = key;
-  }
-  for (int i = n + tid; i < p.keep; i += kBeamThreads) out[i] = 0;
+  if (part == p.parts - 1 && tail > 0 && warp == 0) take_one(p.vocab - tail + lane, lane < tail);
 
-  if (p.normalise) {
-    maxima[tid] = m;
-    __syncthreads();
-    float all = -INFINITY;
-    for (int i = tid % 32; i < kBeamThreads; i += 32) all = fmaxf(all, maxima[i]);
+  // what reaches the floor, one after the other
+  if (tile > 1) floor = fmaxf(floor, block_bound(m, p.keep, kBeamWarps, maxima));
+  static_assert(kBeamCapacity * sizeof(unsigned long long) <= kBeamStages * kBeamTileBytes, "the tiles' place is used");
+  unsigned long long* sorted = reinterpret_cast<unsigned long long*>(beam_tiles);
+  constexpr int kMine = (kBeamStride + 31) / 32;
+  unsigned long long mine[kMine];
+  int left = 0, place[kMine];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    place[i] = -1;
+    if (i * 32 >= held) continue;
+    mine[i] = i * 32 + lane < held ? segment[i * 32 + lane] : 0;
+    const bool in = mine[i] != 0 && beam_key_logit(mine[i]) >= floor;
+    const unsigned int who = __ballot_sync(0xFFFFFFFFu, in);
+    if (in) place[i] = left + __popc(who & ((1u << lane) - 1));
+    left += __popc(who);
+  }
+  float all = m;
+  if constexpr (NORMALISE) {
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+  }
+  if (lane == 0) { counts[warp] = left; maxima[warp] = all; }
+  __syncthreads();
+  int n = 0, from = 0;
+#pragma unroll
+  for (int w = 0; w < kBeamWarps; ++w) {
+    if (w == warp) from = n;
+    n += counts[w];
+    all = fmaxf(all, maxima[w]);
+  }
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+    if (place[i] >= 0) sorted[from + place[i]] = mine[i];
+  if constexpr (NORMALISE) {
     // a thread without a logit above -infinity has a sum of 0, or NaN
-    double s = m == -INFINITY ? static_cast<double>(sum) : static_cast<double>(sum) * exp(static_cast<double>(m) - static_cast<double>(all));
+    double s = m == -INFINITY ? static_cast<double>(sum) : static_cast<double>(sum) * static_cast<double>(exp_of(m - all));
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (tid % 32 == 0) sums[tid / 32] = s;
-    __syncthreads();
+    if (lane == 0) sums[warp] = s;
+  }
+  __syncthreads();
+  const long long item = static_cast<long long>(blockIdx.x) * p.parts + part;
+  if constexpr (NORMALISE) {
     if (tid == 0) {
-      for (int i = 1; i < kBeamThreads / 32; ++i) s += sums[i];
-      p.part_max[blockIdx.x] = all;
-      p.part_sum[blockIdx.x] = s;
+      double s = sums[0];
+      for (int w = 1; w < kBeamWarps; ++w) s += sums[w];
+      p.part_max[item] = all;
+      p.part_sum[item] = s;
     }
+  }
+  if (n > kBeamRanked) {
+    thin_out(sorted, n, p.keep, &counter);
+    n = p.keep;
+  }
+  unsigned long long* out = p.part_keys + item * p.keep;
+  if (tid < n) {
+    const unsigned long long key = sorted[tid];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += sorted[j] > key;
+    if (rank < p.keep) out[rank] = key;
+  } else if (tid < p.keep) {
+    out[tid] = 0;
   }
 }
 
-// One block per search: log-sums of its prefixes, then the best of all parts' candidates.
+// One block per search: log-sums of its prefixes, then the best of all parts' candidates.  A part's candidates are a sorted list
+// of `keep`; a warp merges up to 32 of them by taking the largest head `keep` times, and the first warp merges what the
+// warps found.  What bounds this is the chain of steps, about 0.1 us for each that is kept, so a step is made short: the candidates' values
+// are worked out beforehand, as whole numbers, and a step is one maximum over a warp.
+//
+// Whole numbers that order as the values do; 0 for -infinity and NaN.
+__device__ __forceinline__ unsigned long long beam_order(double value) {
+  if (!(value > -INFINITY)) return 0;
+  const unsigned long long bits = __double_as_longlong(value + 0.0);
+  return bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+__device__ __forceinline__ double beam_ordered_value(unsigned long long order) {
+  return __longlong_as_double(order >> 63 ? order & ~(1ull << 63) : ~order);
+}
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long x) {
+  const unsigned int hi = static_cast<unsigned int>(x >> 32), top = __reduce_max_sync(0xFFFFFFFFu, hi);
+  const unsigned int low = __reduce_max_sync(0xFFFFFFFFu, hi == top ? static_cast<unsigned int>(x) : 0u);
+  return static_cast<unsigned long long>(top) << 32 | low;
+}
+// A candidate of the merge; order is 0 behind the last of a list.
 struct BeamEntry {
-  double value;
-  unsigned long long key;
+  unsigned long long order, key;
   int beam, pad;
 };
-__device__ __forceinline__ bool better(const BeamEntry& a, const BeamEntry& b) {
-  if (a.value != b.value) return a.value > b.value;
-  if (a.beam != b.beam) return a.beam < b.beam;
-  return a.key > b.key;
+// The lane whose entry comes first: by value, then the lower beam, then the larger key; -1 if no lane has one.
+__device__ __forceinline__ int warp_first(const BeamEntry& e) {
+  const unsigned int hi = static_cast<unsigned int>(e.order >> 32), top = __reduce_max_sync(0xFFFFFFFFu, hi);
+  if (top == 0) return -1;                         // of a value above -infinity the upper half is not 0
+  unsigned int who = __ballot_sync(0xFFFFFFFFu, hi == top);
+  if (__popc(who) > 1) {
+    const unsigned int lo = static_cast<unsigned int>(e.order), low = __reduce_max_sync(0xFFFFFFFFu, hi == top ? lo : 0u);
+    bool in = hi == top && lo == low;
+    who = __ballot_sync(0xFFFFFFFFu, in);
+    if (__popc(who) > 1) {
+      const int first = __reduce_min_sync(0xFFFFFFFFu, in ? e.beam : 0x7FFFFFFF);
+      in = in && e.beam == first;
+      const unsigned long long largest = warp_max(in ? e.key : 0ull);
+      who = __ballot_sync(0xFFFFFFFFu, in && e.key == largest);
+    }
+  }
+  return __ffs(who) - 1;
 }
 
-__global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamParams p) {
-  extern __shared__ unsigned long long beam_smem[];
-  __shared__ int count;
-  __shared__ double maxima[kBeamThreads];
-  __shared__ double limit;
-  double* base = reinterpret_cast<double*>(beam_smem);                     // [beams]: score, less the log-sum
-  BeamEntry* list = reinterpret_cast<BeamEntry*>(base + p.beams + p.beams % 2);   // kBeamMergeList + kBeamMergeTile
-  BeamEntry* best = list + kBeamMergeList + kBeamMergeTile;                // keep
-  unsigned char* done = reinterpret_cast<unsigned char*>(best + p.keep);   // [beams]
-  const int tid = threadIdx.x, batch = blockIdx.x;
+// An entry while lists are merged: list * keep + place of where it came from stands for its key.
+struct __align__(16) BeamMerged {
+  unsigned long long order;
+  int beam, from;
+};
+
+// Takes `keep` times the lane's head that comes first; entry(at) is the lane's at-th (order 0 behind its last), and of equal
+// ones of one beam key(from) decides.  taken[n] gets the entries' `from`, -1 behind the last.
+template <typename Entry, typename Key>
+__device__ __forceinline__ void merge_heads(int* taken, int keep, Entry entry, Key key) {
+  const int lane = threadIdx.x % 32;
+  int at = 1, n = 0;
+  BeamMerged e = entry(0), next = entry(1);
+  for (; n < keep; ++n) {
+    const unsigned int hi = static_cast<unsigned int>(e.order >> 32), top = __reduce_max_sync(0xFFFFFFFFu, hi);
+    if (top == 0) break;                           // of a value above -infinity the upper half is not 0
+    unsigned int who = __ballot_sync(0xFFFFFFFFu, hi == top);
+    if ((who & (who - 1)) != 0) {
+      const unsigned int lo = static_cast<unsigned int>(e.order), low = __reduce_max_sync(0xFFFFFFFFu, hi == top ? lo : 0u);
+      bool in = hi == top && lo == low;
+      who = __ballot_sync(0xFFFFFFFFu, in);
+      if ((who & (who - 1)) != 0) {
+        const int first = __reduce_min_sync(0xFFFFFFFFu, in ? e.beam : 0x7FFFFFFF);
+        in = in && e.beam == first;
+        const unsigned long long mine = in ? key(e.from) : 0ull, largest = warp_max(mine);
+        who = __ballot_sync(0xFFFFFFFFu, in && mine == largest);
+      }
+    }
+    if (lane == __ffs(who) - 1) {
+      taken[n] = e.from;
+      e = next;
+      next = entry(++at);
+    }
+  }
+  for (n += lane; n < keep; n += 32) taken[n] = -1;
+}
+
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamParams p) {
+  extern __shared__ __align__(16) unsigned char beam_smem[];
+  constexpr int kWarps = kMergeThreads / 32;
+  const int lists = p.beams * p.parts, entries = lists * p.keep;                  // at most 1024 + 1036 lists
+  const bool merged = entries <= kBeamMergeMost && lists <= 32 * kWarps;
+  BeamMerged* here = reinterpret_cast<BeamMerged*>(beam_smem);                    // [lists][keep], if they fit
+  double* base = reinterpret_cast<double*>(here + (merged ? entries : 0));        // [beams]: score, less the log-sum
+  BeamEntry* found = reinterpret_cast<BeamEntry*>(base + p.beams);                // [1 + warps][keep]: the result, what each warp found;
+  int* taken = reinterpret_cast<int*>(found);                                     // where lists fit, as places in `here`
+  unsigned char* place = reinterpret_cast<unsigned char*>(merged ? static_cast<void*>(taken + (1 + kWarps) * p.keep)
+                                                                 : static_cast<void*>(found + (1 + kWarps) * p.keep));
+  unsigned char* done = place + (merged ? 0 : lists);                             // [beams], behind [lists]: how far each has been taken
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, batch = blockIdx.x;
   grid_dependency_wait();
   grid_dependency_launch();
-  if (tid == 0) { count = 0; limit = -INFINITY; }
-  for (int b = tid / 32; b < p.beams; b += kBeamThreads / 32) {
+  const unsigned long long* far = p.part_keys + static_cast<long long>(batch) * entries;
+  // the first of the keys come in while the log-sums are worked out
+  constexpr int kMine = 4;
+  unsigned long long keys[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) keys[i] = i * kMergeThreads + tid < entries ? far[i * kMergeThreads + tid] : 0;
+  for (int b = warp; b < p.beams; b += kWarps) {
+    const long long part0 = (static_cast<long long>(batch) * p.beams + b) * p.parts;
     const bool ended = p.finished != nullptr && p.finished[batch * p.ld_finished + b] != 0;
     double value = p.scores[batch * p.ld_scores + b];
-    if (p.normalise && !ended) {
-      const long long first = (static_cast<long long>(batch) * p.beams + b) * p.parts;
-      float all = -INFINITY;
-      for (int i = tid % 32; i < p.parts; i += 32) all = fmaxf(all, p.part_max[first + i]);
+    if (p.normalise) {             // an ended prefix has no sums: what is read for it is not used
+      float m = lane < p.parts ? p.part_max[part0 + lane] : -INFINITY, all = m;
+      double s = lane < p.parts ? p.part_sum[part0 + lane] : 0.0;
+      for (int i = lane + 32; i < p.parts; i += 32) all = fmaxf(all, p.part_max[part0 + i]);
 #pragma unroll
       for (int o = 16; o > 0; o /= 2) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
-      double s = 0.0;
-      for (int i = tid % 32; i < p.parts; i += 32) {
-        const float m = p.part_max[first + i];
-        s += m == -INFINITY ? p.part_sum[first + i] : p.part_sum[first + i] * exp(static_cast<double>(m) - static_cast<double>(all));
-      }
+      auto scaled = [&](double sum, float max) {
+        return max == all || max == -INFINITY ? sum : sum * exp(static_cast<double>(max) - static_cast<double>(all));
+      };
+      s = scaled(s, m);
+      for (int i = lane + 32; i < p.parts; i += 32) s += scaled(p.part_sum[part0 + i], p.part_max[part0 + i]);
+      if (p.parts > 1) {
 #pragma unroll
-      for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-      value -= (all == -INFINITY ? 0.0 : static_cast<double>(all)) + log(s);
+        for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      }
+      if (!ended) value -= (all == -INFINITY ? 0.0 : static_cast<double>(all)) + log(s);
     }
-    if (tid % 32 == 0) { base[b] = value; done[b] = ended; }
+    if (lane == 0) { base[b] = value; done[b] = ended; }
   }
   __syncthreads();
 
-  const int per_beam = p.parts * p.keep;
-  const long long entries = static_cast<long long>(p.beams) * per_beam;
-  const unsigned long long* keys = p.part_keys + static_cast<long long>(batch) * entries;
-  double above = -INFINITY;
-  bool at_least = false;                      // candidates are above `above`, or (at_least) at it too
-  for (long long from = 0; from < entries; from += kBeamMergeTile) {
-    BeamEntry e[4];
-    double top = -INFINITY;
+  // entry `at` of list l of beam b; an ended prefix has one entry, in its first list
+  auto work_out = [&](int l, int b, int at, unsigned long long key) {
+    BeamEntry e = {0, key, b, 0};
+    if (done[b]) {
+      if (l == b * p.parts && at == 0) e = {beam_order(base[b]), static_cast<unsigned int>(~p.end_token), b, 0};
+    } else if (key != 0) {
+      e.order = beam_order(base[b] + static_cast<double>(beam_key_logit(key)));
+    }
+    return e;
+  };
+  auto put = [&](int n, unsigned long long order, int beam, int token) {
+    const bool some = order != 0;
+    p.out_scores[batch * p.ld_out_scores + n] = some ? static_cast<float>(beam_ordered_value(order)) : -INFINITY;
+    p.parents[batch * p.ld_parents + n] = some ? beam : -1;
+    p.tokens[batch * p.ld_tokens + n] = some ? token : -1;
+  };
+  if (merged) {
+    auto enter = [&](int e, unsigned long long key) {
+      const int l = e / p.keep, b = l / p.parts;
+      here[e] = {work_out(l, b, e - l * p.keep, key).order, b, e};
+    };
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const long long at = from + u * kBeamThreads + tid;
-      e[u].value = -INFINITY; e[u].key = 0; e[u].beam = 0; e[u].pad = 0;
-      if (at < entries) {
-        const int b = static_cast<int>(at / per_beam);
-        e[u].beam = b;
-        if (done[b]) {
-          if (at % per_beam == 0) {
-            e[u].value = base[b];
-            e[u].key = static_cast<unsigned int>(~p.end_token);
-          }
-        } else {
-          e[u].key = keys[at];
-          if (e[u].key != 0) e[u].value = base[b] + static_cast<double>(beam_key_logit(e[u].key));
-        }
-        if (!(e[u].value > -INFINITY)) e[u].value = -INFINITY;      // NaN is no candidate
-      }
-      top = fmax(top, e[u].value);
-    }
-    if (from == 0) {
-      maxima[tid] = top;
-      __syncthreads();
-      int rank = 0;
-#pragma unroll 8
-      for (int i = 0; i < kBeamThreads; ++i) rank += maxima[i] > top || (maxima[i] == top && i < tid);
-      if (rank == p.keep - 1) limit = top;
-      __syncthreads();
-      above = limit;
-      at_least = above > -INFINITY;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (e[u].value > above || (at_least && e[u].value == above)) list[atomicAdd(&count, 1)] = e[u];
+    for (int i = 0; i < kMine; ++i)
+      if (i * kMergeThreads + tid < entries) enter(i * kMergeThreads + tid, keys[i]);
+    for (int e = kMine * kMergeThreads + tid; e < entries; e += kMergeThreads) enter(e, far[e]);
     __syncthreads();
-    const int n = count;
-    const bool last = from + kBeamMergeTile >= entries;
-    if (n > kBeamMergeList || last) {
-      for (int i = tid; i < n; i += kBeamThreads) {
-        const BeamEntry mine = list[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += better(list[j], mine);
-        if (rank < p.keep) best[rank] = mine;
-      }
+    auto key = [&](int from) { return far[from]; };        // (an ended prefix has one entry: its key is not asked for)
+    const BeamMerged none = {0, 0, -1};
+    const int warps = (lists + 31) / 32;
+    int* const mine = taken + (warps > 1 ? (1 + warp) * p.keep : 0);
+    if (warp < warps) {
+      const int first = lists * warp / warps, last = lists * (warp + 1) / warps, l = first + lane;
+      merge_heads(mine, p.keep, [&](int at) { return l < last && at < p.keep ? here[l * p.keep + at] : none; }, key);
+    }
+    if (warps > 1) {
       __syncthreads();
-      const int kept = min(n, p.keep);
-      if (!last) {
-        for (int i = tid; i < kept; i += kBeamThreads) list[i] = best[i];
-        if (tid == 0) count = kept;
-        if (kept == p.keep) { above = best[kept - 1].value; at_least = true; }
-      } else {
-        for (int i = tid; i < p.keep; i += kBeamThreads) {
-          const bool some = i < kept;
-          p.out_scores[batch * p.ld_out_scores + i] = some ? static_cast<float>(best[i].value) : -INFINITY;
-          p.parents[batch * p.ld_parents + i] = some ? best[i].beam : -1;
-          p.tokens[batch * p.ld_tokens + i] = some ? beam_key_token(best[i].key) : -1;
-        }
+      if (warp == 0) {
+        const int* theirs = taken + (1 + lane) * p.keep;
+        merge_heads(taken, p.keep, [&](int at) {
+          const int from = lane < warps && at < p.keep ? theirs[at] : -1;
+          return from >= 0 ? here[from] : none;
+        }, key);
       }
     }
-    __syncthreads();
+    __syncwarp();
+    if (warp == 0)
+      for (int n = lane; n < p.keep; n += 32) {
+        const int from = taken[n];
+        const BeamMerged e = from >= 0 ? here[from] : none;
+        put(n, e.order, e.beam, from < 0 ? -1 : done[e.beam] ? p.end_token : beam_key_token(far[from]));
+      }
+    return;
   }
+
+  // More candidates than shared memory holds: the warps share the lists, a warp takes the largest head of its own `keep` times, and
+  // the first merges what they found.
+  auto entry_of = [&](int l, int b, int at) {
+    return at < p.keep ? work_out(l, b, at, far[static_cast<long long>(l) * p.keep + at]) : BeamEntry{0, 0, b, 0};
+  };
+  const BeamEntry none = {0, 0, -1, 0};
+  BeamEntry* result = found;
+  found += p.keep;
+  const int first = static_cast<int>(static_cast<long long>(lists) * warp / kWarps), last = static_cast<int>(static_cast<long long>(lists) * (warp + 1) / kWarps);
+  for (int l = first + lane; l < last; l += 32) place[l] = 0;
+  BeamEntry best;
+  int from;
+  auto look = [&] {                // the lane's first entry
+    best = none;
+    from = -1;
+    for (int l = first + lane; l < last; l += 32) {
+      const BeamEntry e = entry_of(l, l / p.parts, place[l]);
+      if (e.order > best.order || (e.order != 0 && e.order == best.order && e.beam == best.beam && e.key > best.key)) { best = e; from = l; }
+    }
+  };
+  look();
+  int n = 0;
+  for (; n < p.keep; ++n) {
+    const int who = warp_first(best);
+    if (who < 0) break;
+    if (lane == who) {
+      found[warp * p.keep + n] = best;
+      ++place[from];
+      look();
+    }
+  }
+  for (n += lane; n < p.keep; n += 32) found[warp * p.keep + n] = none;
+  __syncthreads();
+  if (warp > 0) return;
+  int at = 0;                      // lane w: how far list w of `found` has been taken
+  BeamEntry e = lane < kWarps ? found[lane * p.keep] : none;
+  for (int i = 0; i < p.keep; ++i) {
+    const int who = warp_first(e);
+    if (who < 0 ? lane == 0 : lane == who) result[i] = e;
+    if (lane == who) e = ++at < p.keep ? found[lane * p.keep + at] : none;
+  }
+  __syncwarp();
+  for (int i = lane; i < p.keep; i += 32) put(i, result[i].order, result[i].beam, beam_key_token(result[i].key));
 }
 
 }  // namespace cuasr_b200

@@ -2,6 +2,8 @@
 // arguments and plans the launches.  Also what decode.cu shares with abi.cu.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_runtime.h>
 
 #include "../../include/cuasr_b200_decode.h"
@@ -16,6 +18,19 @@ struct DeviceInfo {
 bool current_device_info(DeviceInfo* out);
 // Adds to cuasr_b200_launch_count and names the call for cuasr_b200_last_kernel and cuasr_b200_last_route (abi.cu).
 void note_launches(const char* kernel, int count);
+
+// Opts a kernel in to `bytes` of dynamic shared memory (with its static more than 48 KB), once per device; `done` belongs
+// to the kernel.
+inline cudaError_t allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return err;
+}
 
 cudaError_t launch_q4(const cuasr_b200_q4_args_t& args, const DeviceInfo& dev, int* launches);
 

@@ -1,26 +1,13 @@
 // Launchers of q4_kernel; instantiated by the number of columns in the inst_q4_*.cu files so that they compile in parallel.
 #pragma once
 
-#include <atomic>
-
+#include "decode_launch.h"
 #include "q4_product.cuh"
 
 namespace cuasr_b200 {
 
 // a block has 1 KB of static shared memory and 1 KB that the driver keeps
 constexpr int kQ4SmemPerSm = 228 * 1024, kQ4SmemPerBlock = kQ4SmemPerSm - 2048;
-
-// Opts a kernel in to more than 48 KB of shared memory, once per device.
-inline cudaError_t allow_shared_memory(const void* kernel, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err != cudaSuccess) return err;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemPerBlock);
-  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-  return err;
-}
 
 struct Q4Launch {
   int grid_x, grid_y, smem;
@@ -31,7 +18,7 @@ template <bool BF16, int NT, int LW, bool TMA, bool ZEROS>
 cudaError_t launch_q4_kernel(const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
   static std::atomic<uint64_t> allowed{0};
   auto kernel = q4_kernel<BF16, NT, LW, TMA, ZEROS>;
-  const cudaError_t err = allow_shared_memory(reinterpret_cast<const void*>(kernel), allowed);
+  const cudaError_t err = allow_shared_memory(reinterpret_cast<const void*>(kernel), kQ4SmemPerBlock, allowed);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(l.grid_x), static_cast<unsigned>(l.grid_y));
