@@ -7,17 +7,17 @@ namespace cuasr_b200 {
 namespace {
 
 struct Q4Plan {
-  int parts = 0, slices = 1, panel_steps = 0, stages = 0, grid = 0, sum_bytes = 0, xsum_bytes = 0, smem = 0;
+  int warps = 0, parts = 0, slices = 1, panel_steps = 0, stages = 0, grid = 0, sum_bytes = 0, xsum_bytes = 0, smem = 0;
 };
 // What the shape of X and of the groups makes of a block.
 struct Q4Shape {
-  int columns, column_tiles, warps, groups_per_step, stage_bytes;
+  int columns, column_tiles, groups_per_step, stage_bytes;
 };
 
 // Shared memory of a block: stages, sums, X of a panel and what is read behind it.
 void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
-  plan->sum_bytes = s.warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * kQ4SumStride * 4;
-  const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = s.warps * s.stage_bytes;
+  plan->sum_bytes = plan->warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * kQ4SumStride * 4;
+  const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = plan->warps * s.stage_bytes;
   const int per_step = 512 * s.columns + 4 * s.groups_per_step * ((s.columns + 1) / 2 * 2), room = kQ4SmemPerBlock - fixed;
   int panel = slice_steps;
   if (panel > (room - 2 * all_stages) / per_step) panel = (room - 2 * all_stages) / per_step / plan->parts * plan->parts;
@@ -30,29 +30,33 @@ void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
 Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, int sms) {
   Q4Plan best;
   double best_cost = 0;
-  for (int parts = 1; parts <= shape.warps && parts <= 8; parts *= 2)
-    for (int s = 1; s <= kQ4MaxSlices && (s == 1 || s <= steps); s *= 2) {
-      Q4Plan plan;
-      plan.parts = parts;
-      plan.slices = s;
-      const int workers = shape.warps / parts, slice_steps = (steps + s - 1) / s;
-      fit(&plan, slice_steps, shape);
-      if (plan.panel_steps <= 0) continue;
-      const int blocks = std::max(1, std::min((units + workers - 1) / workers, std::max(1, sms / s)));
-      const double rounds = static_cast<double>(((units + workers - 1) / workers + blocks - 1) / blocks) * passes;
-      // In microseconds, from measurements between 1024 x 1024 and 128000 x 4096: a warp's step 1.7 with all warps at it, a
-      // worker's sums 1.3, a cluster's 2 more; X laid out by a block 0.5 for a step of all its columns' warps.  (One row,
-      // 14336 x 4096: 12.4 with four parts, 13.9 with eight, 17 with two.  Eight rows, 128000 x 4096: 63 with one part, 65 with
-      // four.  Thirty-two rows, 8192 x 8192: 38 with four slices of one part, 48 with two of two, 84 with two parts alone.)
-      const double restaged = plan.panel_steps < slice_steps ? rounds : passes;
-      const double cost = rounds * ((slice_steps + parts - 1) / parts * 1.7 + (parts > 1 ? 1.3 : 1.0) + (s > 1 ? 2.0 : 0.0)) +
-                          restaged * slice_steps * shape.columns * 0.5 / shape.warps;
-      if (best.smem == 0 || cost < best_cost) {
-        best_cost = cost;
-        plan.grid = blocks * s;
-        best = plan;
+  for (int warps = shape.column_tiles == 1 ? 16 : 8; warps >= 8; warps /= 2)
+    for (int parts = 1; parts <= 8; parts *= 2)
+      for (int s = 1; s <= kQ4MaxSlices && (s == 1 || s <= steps); s *= 2) {
+        Q4Plan plan;
+        plan.warps = warps;
+        plan.parts = parts;
+        plan.slices = s;
+        const int workers = warps / parts, slice_steps = (steps + s - 1) / s;
+        fit(&plan, slice_steps, shape);
+        if (plan.panel_steps <= 0) continue;
+        const int blocks = std::max(1, std::min((units + workers - 1) / workers, std::max(1, sms / s)));
+        const double rounds = static_cast<double>(((units + workers - 1) / workers + blocks - 1) / blocks) * passes;
+        // In microseconds, from measurements between 1024 x 1024 and 128000 x 4096: a warp's step with all warps at it 1.7 (16 of
+        // them; 1.4 with eight, 2 for 32 columns), a worker's sums 1.3, a cluster's 2 more; X laid out by a block 0.5 for a step of
+        // all its columns' warps.  (One row, 14336 x 4096: 12.4 with four parts, 13.9 with eight, 17 with two.  Eight rows, 128000
+        // x 4096: 63 with one part, 65 with four.  Sixteen: 97 with eight warps, whose shared memory holds X, 198 with
+        // sixteen.  Thirty-two rows, 8192 x 8192: 38 with four slices of one part, 48 with two of two, 84 with two parts.)
+        const double step = shape.column_tiles == 4 ? 2.0 : warps == 16 ? 1.7 : 1.4;
+        const double restaged = plan.panel_steps < slice_steps ? rounds : passes;
+        const double cost = rounds * ((slice_steps + parts - 1) / parts * step + (parts > 1 ? 1.3 : 1.0) + (s > 1 ? 2.0 : 0.0)) +
+                            restaged * slice_steps * shape.columns * 0.5 / warps;
+        if (best.smem == 0 || cost < best_cost) {
+          best_cost = cost;
+          plan.grid = blocks * s;
+          best = plan;
+        }
       }
-    }
   return best;
 }
 
@@ -100,15 +104,16 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
   const int steps = (a.k + kQ4Step - 1) / kQ4Step;
   CUtensorMap map = {};
   const bool tma = weight_map(&map, a);
-  const Q4Shape shape = {columns, nt, nt == 4 ? kQ4Warps<4> : kQ4Warps<1>, 8 / lw, tma ? kQ4Stage<true> : kQ4Stage<false>};
+  const Q4Shape shape = {columns, nt, 8 / lw, tma ? kQ4Stage<true> : kQ4Stage<false>};
   p.units = (a.n - 1) / kQ4Rows + 1;
   const Q4Plan plan = plan_q4(p.units, steps, passes, shape, dev.sms);
   if (plan.smem == 0) return cudaErrorInvalidValue;      // no launch fits: never for one block per SM and one slice
   p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.stages = plan.stages; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
   const Q4Launch l = {plan.grid, passes, plan.smem, static_cast<cudaStream_t>(a.stream)};
-  const cudaError_t err = nt == 1   ? launch_q4_columns<1>(lw, tma, map, p, l)
-                          : nt == 2 ? launch_q4_columns<2>(lw, tma, map, p, l)
-                                    : launch_q4_columns<4>(lw, tma, map, p, l);
+  const cudaError_t err = nt == 4                ? launch_q4_columns<4, 8>(lw, tma, map, p, l)
+                          : nt == 2          ? launch_q4_columns<2, 8>(lw, tma, map, p, l)
+                          : plan.warps == 16 ? launch_q4_columns<1, 16>(lw, tma, map, p, l)
+                                             : launch_q4_columns<1, 8>(lw, tma, map, p, l);
   if (err == cudaSuccess) ++*launches;
   return err;
 }

@@ -14,15 +14,15 @@ struct Q4Launch {
   cudaStream_t stream;
 };
 
-template <bool BF16, int NT, int LW, bool TMA, bool ZEROS>
+template <bool BF16, int NT, int WARPS, int LW, bool TMA, bool ZEROS>
 cudaError_t launch_q4_kernel(const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
   static std::atomic<uint64_t> allowed{0};
-  auto kernel = q4_kernel<BF16, NT, LW, TMA, ZEROS>;
+  auto kernel = q4_kernel<BF16, NT, WARPS, LW, TMA, ZEROS>;
   const cudaError_t err = allow_shared_memory(reinterpret_cast<const void*>(kernel), kQ4SmemPerBlock, allowed);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(l.grid_x), static_cast<unsigned>(l.grid_y));
-  config.blockDim = dim3(32 * kQ4Warps<NT>);
+  config.blockDim = dim3(32 * WARPS);
   config.dynamicSmemBytes = static_cast<size_t>(l.smem);
   config.stream = l.stream;
   cudaLaunchAttribute attr[2];
@@ -36,12 +36,12 @@ cudaError_t launch_q4_kernel(const CUtensorMap& map, const Q4Params& p, const Q4
   return cudaLaunchKernelEx(&config, kernel, map, p);
 }
 
-template <int NT>
+template <int NT, int WARPS>
 cudaError_t launch_q4_columns(int lw, bool tma, const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
   const bool zeros = p.zeros != nullptr, bf16 = p.type_x != CUASR_F16;
 #define Q4_CASE(L, V, Z)                                                            \
   if (lw == L && tma == V && zeros == Z)                                            \
-    return bf16 ? launch_q4_kernel<true, NT, L, V, Z>(map, p, l) : launch_q4_kernel<false, NT, L, V, Z>(map, p, l);
+    return bf16 ? launch_q4_kernel<true, NT, WARPS, L, V, Z>(map, p, l) : launch_q4_kernel<false, NT, WARPS, L, V, Z>(map, p, l);
 #define Q4_CASES(L) Q4_CASE(L, false, false) Q4_CASE(L, true, false) Q4_CASE(L, false, true) Q4_CASE(L, true, true)
   Q4_CASES(1) Q4_CASES(2) Q4_CASES(4)
 #undef Q4_CASES
@@ -49,8 +49,9 @@ cudaError_t launch_q4_columns(int lw, bool tma, const CUtensorMap& map, const Q4
   return cudaErrorInvalidValue;
 }
 
-extern template cudaError_t launch_q4_columns<1>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
-extern template cudaError_t launch_q4_columns<2>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
-extern template cudaError_t launch_q4_columns<4>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<1, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<1, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<2, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<4, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
 
 }  // namespace cuasr_b200

@@ -42,7 +42,7 @@ constexpr int kQ4Pitch = kQ4Step / 2 + 4;     // bytes between rows of a stage t
 template <bool TMA> constexpr int kQ4Stage = kQ4Rows * (TMA ? kQ4Step / 2 : kQ4Pitch);
 constexpr int kQ4MaxStages = 4;
 constexpr int kQ4MaxSlices = 4;               // blocks of a cluster that share k
-template <int NT> constexpr int kQ4Warps = NT == 4 ? 8 : 16;       // the sums of 32 columns leave registers for eight
+// Warps of a block: 16, or 8 where the sums of more than eight columns take the registers or X the shared memory.
 constexpr int kQ4SumStride = kQ4Rows + 4;     // floats between columns of a warp's sums: no bank twice
 template <int NT> constexpr int kQ4Buffer = NT * 8 * kQ4SumStride; // floats of a warp's sums
 // X is read eight columns at a time: what lies behind a panel's last word has to be there.
@@ -166,7 +166,22 @@ __device__ __forceinline__ void copy_word(const Q4Params& p, unsigned char* stag
 }
 __device__ __forceinline__ void copy_step(const Q4Params& p, unsigned char* stage, long long first_row, int step, int lane, int row_bytes,
                                           const unsigned char* last) {
-#pragma unroll 4
+  const unsigned char* q = p.W + first_row * p.ldw + static_cast<long long>(step) * (kQ4Step / 2);
+  if (first_row + kQ4Rows <= p.n && q - 3 >= p.W && q + (kQ4Rows - 1) * p.ldw + kQ4Step / 2 + 4 <= last) {
+    // every word lies inside the operand; what lies behind a row's end meets zeros of X
+    const uint32_t to = smem_u32(stage) + lane * 4;
+#pragma unroll 8
+    for (int r = 0; r < kQ4Rows; ++r) {
+      const unsigned char* a = q - (reinterpret_cast<uintptr_t>(q) & 3) + lane * 4;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + r * kQ4Pitch), "l"(a) : "memory");
+      q += p.ldw;
+    }
+    const unsigned char* mine = p.W + (first_row + lane) * p.ldw + static_cast<long long>(step) * (kQ4Step / 2);
+    const unsigned char* a = mine - (reinterpret_cast<uintptr_t>(mine) & 3) + 128;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(stage) + lane * kQ4Pitch + 128), "l"(a) : "memory");
+    return;
+  }
+#pragma unroll 1
   for (int r = 0; r < kQ4Rows; ++r) copy_word(p, stage, first_row + r, step, r, lane, row_bytes, last);
   copy_word(p, stage, first_row + lane, step, lane, 32, row_bytes, last);
 }
@@ -312,17 +327,17 @@ __device__ __forceinline__ void worker_barrier(int worker, int warps) {
 }
 
 // NT tiles of eight columns of X.
-template <bool BF16, int NT, int LW, bool TMA, bool ZEROS>
-__global__ void __launch_bounds__(32 * kQ4Warps<NT>, 1)
+template <bool BF16, int NT, int WARPS, int LW, bool TMA, bool ZEROS>
+__global__ void __launch_bounds__(32 * WARPS, 1)
 q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Params p) {
   extern __shared__ __align__(1024) unsigned char q4_smem[];
-  constexpr int kThreads = 32 * kQ4Warps<NT>, RT = kQ4Rows / 16;
-  __shared__ uint64_t full[kQ4Warps<NT>][kQ4MaxStages];
+  constexpr int kThreads = 32 * WARPS, RT = kQ4Rows / 16;
+  __shared__ uint64_t full[WARPS][kQ4MaxStages];
   __shared__ unsigned int abandoned;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
-  const int parts = p.parts, part_of = warp % parts, local = warp / parts, workers_here = kQ4Warps<NT> / parts;
+  const int parts = p.parts, part_of = warp % parts, local = warp / parts, workers_here = WARPS / parts;
   unsigned char* stages = q4_smem + warp * p.stages * kQ4Stage<TMA>;
-  float* all_sums = reinterpret_cast<float*>(q4_smem + kQ4Warps<NT> * p.stages * kQ4Stage<TMA>);
+  float* all_sums = reinterpret_cast<float*>(q4_smem + WARPS * p.stages * kQ4Stage<TMA>);
   const int buffers = max(parts - 1, 1);                   // of a worker
   float* sums = all_sums + local * buffers * kQ4Buffer<NT>;
   float* xsums = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(all_sums) + p.sum_bytes);
