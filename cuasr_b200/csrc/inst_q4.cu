@@ -7,7 +7,7 @@ namespace cuasr_b200 {
 namespace {
 
 struct Q4Plan {
-  int warps = 0, parts = 0, slices = 1, panel_steps = 0, stages = 0, grid = 0, sum_bytes = 0, xsum_bytes = 0, smem = 0;
+  int warps = 0, parts = 0, slices = 1, panel_steps = 0, grid = 0, sum_bytes = 0, xsum_bytes = 0, smem = 0;
 };
 // What the shape of X and of the groups makes of a block.
 struct Q4Shape {
@@ -17,14 +17,13 @@ struct Q4Shape {
 // Shared memory of a block: stages, sums, X of a panel and what is read behind it.
 void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
   plan->sum_bytes = plan->warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * kQ4SumStride * 4;
-  const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = plan->warps * s.stage_bytes;
+  const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = kQ4Stages * plan->warps * s.stage_bytes;
   const int per_step = 512 * s.columns + 4 * s.groups_per_step * ((s.columns + 1) / 2 * 2), room = kQ4SmemPerBlock - fixed;
   int panel = slice_steps;
-  if (panel > (room - 2 * all_stages) / per_step) panel = (room - 2 * all_stages) / per_step / plan->parts * plan->parts;
+  if (panel > (room - all_stages) / per_step) panel = (room - all_stages) / per_step / plan->parts * plan->parts;
   plan->panel_steps = panel;
-  plan->stages = 2;                  // three measured slower: 128000 x 4096 read alone in 53 us instead of 45
   plan->xsum_bytes = (4 * s.groups_per_step * ((s.columns + 1) / 2 * 2) * panel + 15) / 16 * 16;
-  plan->smem = fixed - 16 + plan->xsum_bytes + panel * 512 * s.columns + plan->stages * all_stages;
+  plan->smem = fixed - 16 + plan->xsum_bytes + panel * 512 * s.columns + all_stages;
 }
 
 Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, int sms) {
@@ -108,7 +107,7 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
   p.units = (a.n - 1) / kQ4Rows + 1;
   const Q4Plan plan = plan_q4(p.units, steps, passes, shape, dev.sms);
   if (plan.smem == 0) return cudaErrorInvalidValue;      // no launch fits: never for one block per SM and one slice
-  p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.stages = plan.stages; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
+  p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
   const Q4Launch l = {plan.grid, passes, plan.smem, static_cast<cudaStream_t>(a.stream)};
   const cudaError_t err = nt == 4                ? launch_q4_columns<4, 8>(lw, tma, map, p, l)
                           : nt == 2          ? launch_q4_columns<2, 8>(lw, tma, map, p, l)
