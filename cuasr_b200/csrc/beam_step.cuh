@@ -4,8 +4,9 @@
 //
 // Within a prefix the values order as its logits do, so one pass over the logits finds both the sum and the prefix's own
 // `keep` best; the searches' best are then chosen among those.  The floor is the logits' bytes at the memory's rate, which
-// leaves about eleven instructions of a lane for a 16-bit logit and twice as many for a 32-bit one; so exponentials are worked out in pairs, and a logit is otherwise only part of a maximum, which is
-// compared with a bound that nearly all threads stay below.  The bound comes from the threads' own maxima and is taken
+// leaves about eleven instructions of a lane for a 16-bit logit and twice as many for a 32-bit one; so exponentials are worked
+// out in pairs, and a logit is otherwise only part of a maximum, which is compared with a bound that nearly all threads stay
+// below.  The bound comes from the threads' own maxima and is taken
 // again after 1, 2, 4, ... tiles; a row of 16 tiles then has about seven candidates for each that is kept, which every warp
 // collects by itself and which are sorted once, at the row's end.
 #pragma once
@@ -23,7 +24,7 @@ constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamSegment = 128;                               // candidates that a warp can hold after a tile ...
 constexpr int kBeamStride = kBeamSegment + 8;                   // ... and the few logits behind the last
 constexpr int kBeamCapacity = kBeamWarps * kBeamStride;
-constexpr int kBeamRanked = kBeamThreads;                                // up to so many are sorted by comparing all with all
+constexpr int kBeamRanked = kBeamThreads;                       // up to so many are sorted by comparing all with all
 constexpr int kMergeThreads = 256;
 constexpr int kBeamMergeMost = 8192;                            // candidates that are merged in shared memory
 
@@ -203,8 +204,8 @@ __device__ __noinline__ void thin_out(unsigned long long* keys, int n, int keep,
   __syncthreads();
 }
 
-// A block has part blockIdx.y of row blockIdx.x: of its vectors `chunk`, and the few logits in front with the first part, those behind
-// with the last.
+// A block has part blockIdx.y of row blockIdx.x: `chunk` of its vectors, and with the first part the few logits in front of
+// them, with the last those behind.
 template <typename T, bool NORMALISE>
 __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(const BeamParams p) {
   extern __shared__ __align__(128) uint4 beam_tiles[];            // kBeamStages tiles
@@ -403,8 +404,8 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
 
 // One block per search: log-sums of its prefixes, then the best of all parts' candidates.  A part's candidates are a sorted list
 // of `keep`; a warp merges up to 32 of them by taking the largest head `keep` times, and the first warp merges what the
-// warps found.  What bounds this is the chain of steps, about 0.1 us for each that is kept, so a step is made short: the candidates' values
-// are worked out beforehand, as whole numbers, and a step is one maximum over a warp.
+// warps found.  What bounds this is the chain of steps, about 0.1 us for each that is kept, so a step is made short: the
+// candidates' values are worked out beforehand, as whole numbers, and a step is one maximum over a warp.
 //
 // Whole numbers that order as the values do; 0 for -infinity and NaN.
 __device__ __forceinline__ unsigned long long beam_order(double value) {
@@ -581,8 +582,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
     return;
   }
 
-  // More candidates than shared memory holds: the warps share the lists, a warp takes the largest head of its own `keep` times, and
-  // the first merges what they found.
+  // More candidates than shared memory holds: the warps share the lists, a warp takes the largest head of its own `keep`
+  // times, and the first merges what they found.
   auto entry_of = [&](int l, int b, int at) {
     return at < p.keep ? work_out(l, b, at, far[static_cast<long long>(l) * p.keep + at]) : BeamEntry{0, 0, b, 0};
   };

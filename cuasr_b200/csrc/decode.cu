@@ -45,7 +45,7 @@ int validate_q4(const cuasr_b200_q4_args_t* a) {
   if (!aligned(a->X, element_bytes(a->dtype_x)) || !aligned(a->Y, element_bytes(a->dtype_y)) ||
       !aligned(a->scales, element_bytes(a->dtype_scale)))
     return CUASR_STATUS_ERROR_MISALIGNED_OPERAND;
-  return CUASR_STATUS_SUCCESS;
+  return q4_fits(*a) ? CUASR_STATUS_SUCCESS : CUASR_STATUS_ERROR_NOT_SUPPORTED;
 }
 
 int validate_beam_sizes(const cuasr_b200_beam_args_t* a) {
@@ -109,10 +109,11 @@ int validate_reorder(const cuasr_b200_reorder_args_t* a) {
           to[d] > INT64_MAX / 2 / std::max<int64_t>(1, written[d]) / 4)
         return CUASR_STATUS_ERROR_INVALID_PROBLEM;
     int64_t src_extent = 0, dst_extent = 0;
-    (void)lies_apart(from, read, s.bytes, &src_extent);
+    const bool src_apart = lies_apart(from, read, s.bytes, &src_extent);
     if (!lies_apart(to, written, s.bytes, &dst_extent)) return CUASR_STATUS_ERROR_INVALID_PROBLEM;
     if (s.src == s.dst && std::equal(from, from + 4, to)) {
-      if (a->keep > a->beams) return CUASR_STATUS_ERROR_INVALID_PROBLEM;
+      // rows that are only read must not be another search's that are written
+      if (a->keep > a->beams || !src_apart) return CUASR_STATUS_ERROR_INVALID_PROBLEM;
       if (a->keep > CUASR_B200_REORDER_MAX_IN_PLACE) return CUASR_STATUS_ERROR_NOT_SUPPORTED;
     } else {
       const char *x = static_cast<const char*>(s.src), *y = static_cast<const char*>(s.dst);
@@ -121,7 +122,7 @@ int validate_reorder(const cuasr_b200_reorder_args_t* a) {
     for (int j = 0; j < i; ++j)
       if (a->states[j].dst == s.dst || a->states[j].dst == s.src || a->states[j].src == s.dst) return CUASR_STATUS_ERROR_INVALID_PROBLEM;
   }
-  return CUASR_STATUS_SUCCESS;
+  return reorder_fits(*a) ? CUASR_STATUS_SUCCESS : CUASR_STATUS_ERROR_NOT_SUPPORTED;
 }
 
 // Runs `launch` on the device of the call.
@@ -134,7 +135,6 @@ int run_on_device(const Args& args, const char* kernel, Launch launch) {
   int launches = 0;
   const cudaError_t err = launch(args, dev, &launches);
   note_launches(kernel, launches);
-  if (err == cudaErrorInvalidConfiguration) return CUASR_STATUS_ERROR_NOT_SUPPORTED;
   return err == cudaSuccess ? CUASR_STATUS_SUCCESS : CUASR_STATUS_ERROR_INTERNAL;
 }
 

@@ -32,6 +32,8 @@ inline cudaError_t allow_shared_memory(const void* kernel, int bytes, std::atomi
   return err;
 }
 
+// Whether the sizes of valid arguments are within the kernel's.
+bool q4_fits(const cuasr_b200_q4_args_t& args);
 cudaError_t launch_q4(const cuasr_b200_q4_args_t& args, const DeviceInfo& dev, int* launches);
 
 // Into how many parts the vocabulary of every prefix is cut; by the sizes alone, so that the workspace does not depend
@@ -40,6 +42,7 @@ int beam_parts(const cuasr_b200_beam_args_t& args);
 size_t beam_workspace_bytes(const cuasr_b200_beam_args_t& args);
 cudaError_t launch_beam(const cuasr_b200_beam_args_t& args, const DeviceInfo& dev, int* launches);
 
+bool reorder_fits(const cuasr_b200_reorder_args_t& args);
 cudaError_t launch_reorder(const cuasr_b200_reorder_args_t& args, const DeviceInfo& dev, int* launches);
 
 }  // namespace cuasr_b200

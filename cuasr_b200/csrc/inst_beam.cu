@@ -11,7 +11,8 @@ namespace cuasr_b200 {
 int beam_parts(const cuasr_b200_beam_args_t& a) {
   const long long rows = static_cast<long long>(a.batch) * a.beams;
   const int tile = kBeamThreads * kBeamVectors * (a.dtype == CUASR_F32 ? 4 : 8);
-  const long long fill = kBeamBlocks * 148 / rows, tiles = (a.vocab + tile - 1) / tile, room = std::min(kBeamMergeMost / (a.beams * a.keep), kMergeThreads / a.beams);
+  const long long fill = kBeamBlocks * 148 / rows, tiles = (static_cast<long long>(a.vocab) + tile - 1) / tile;
+  const long long room = std::min(kBeamMergeMost / (a.beams * a.keep), kMergeThreads / a.beams);
   return static_cast<int>(std::max(1LL, std::min({fill, tiles, room, 32LL})));
 }
 

@@ -14,7 +14,7 @@ struct Q4Shape {
   int columns, column_tiles, groups_per_step, stage_bytes;
 };
 
-// Shared memory of a block: stages, sums, X of a panel and what is read behind it.
+// Shared memory of a block: stages, sums, X of a panel and what is read behind it (X is read eight columns at a time).
 void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
   plan->sum_bytes = plan->warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * kQ4SumStride * 4;
   const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = kQ4Stages * plan->warps * s.stage_bytes;
@@ -79,6 +79,14 @@ bool weight_map(CUtensorMap* map, const cuasr_b200_q4_args_t& a) {
 
 }  // namespace
 
+// Passes over the weights, each with up to 32 columns of X: as many rows, or ten of 32 bits.
+static int q4_passes(const cuasr_b200_q4_args_t& a) { return (a.m - 1) / (a.dtype_x == CUASR_F32 ? 10 : 32) + 1; }
+
+bool q4_fits(const cuasr_b200_q4_args_t& a) {
+  // row and step numbers stay 32-bit up to a grid's stride behind the last
+  return a.n <= 0x7FFE0000 && a.k <= 0x7FFE0000 && q4_passes(a) <= 65535;
+}
+
 cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int* launches) {
   Q4Params p = {};
   p.X = a.X; p.ldx = a.ldx; p.W = a.W; p.ldw = a.ldw; p.scales = a.scales; p.ld_scales = a.ld_scales;
@@ -90,11 +98,7 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
     if (a.group == 1 << b) p.group_shift = b;
   p.type_x = a.dtype_x; p.type_y = a.dtype_y; p.type_scale = a.dtype_scale;
   p.status = dev.status;
-  // offsets inside a tile are 32-bit
-  if (a.ld_scales > (1 << 24) || a.ld_zeros > (1 << 24) || a.n > 0x7FFFFFFF - 1024 || a.k > 0x7FFFFFFF - kQ4Step) return cudaErrorInvalidConfiguration;
-  const int parts = a.dtype_x == CUASR_F32 ? 3 : 1, most_rows = 32 / parts;
-  const int passes = (a.m - 1) / most_rows + 1;
-  if (passes > 65535) return cudaErrorInvalidConfiguration;
+  const int parts = a.dtype_x == CUASR_F32 ? 3 : 1, passes = q4_passes(a);
   p.rows = (a.m - 1) / passes + 1;
   const int columns = p.rows * parts, nt = columns <= 8 ? 1 : columns <= 16 ? 2 : 4;
   const size_t es = a.dtype_x == CUASR_F32 ? 4 : 2;
@@ -109,7 +113,7 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
   if (plan.smem == 0) return cudaErrorInvalidValue;      // no launch fits: never for one block per SM and one slice
   p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
   const Q4Launch l = {plan.grid, passes, plan.smem, static_cast<cudaStream_t>(a.stream)};
-  const cudaError_t err = nt == 4                ? launch_q4_columns<4, 8>(lw, tma, map, p, l)
+  const cudaError_t err = nt == 4          ? launch_q4_columns<4, 8>(lw, tma, map, p, l)
                           : nt == 2          ? launch_q4_columns<2, 8>(lw, tma, map, p, l)
                           : plan.warps == 16 ? launch_q4_columns<1, 16>(lw, tma, map, p, l)
                                              : launch_q4_columns<1, 8>(lw, tma, map, p, l);

@@ -66,19 +66,21 @@ cudaError_t launch_some(const ReorderParams& p, unsigned int grid, cudaStream_t 
 
 }  // namespace
 
+bool reorder_fits(const cuasr_b200_reorder_args_t& a) {
+  ReorderState r;
+  for (int i = 0; i < a.n_states; ++i)
+    if (!plan_state(a.states[i], a, &r)) return false;
+  return true;
+}
+
 cudaError_t launch_reorder(const cuasr_b200_reorder_args_t& a, const DeviceInfo& dev, int* launches) {
   ReorderParams p = {};
   p.parents = a.parents; p.ld_parents = a.ld_parents; p.lengths = a.lengths; p.status = dev.status;
   p.beams = a.beams; p.keep = a.keep;
-  // all states are planned before the first launch: a call is refused whole
-  for (int i = 0; i < a.n_states; ++i) {
-    ReorderState r;
-    if (!plan_state(a.states[i], a, &r)) return cudaErrorInvalidConfiguration;
-  }
   unsigned long long grid = 0;
   for (int i = 0; i < a.n_states; ++i) {
     ReorderState r;
-    (void)plan_state(a.states[i], a, &r);
+    if (!plan_state(a.states[i], a, &r)) return cudaErrorInvalidValue;     // reorder_fits() was asked before
     const unsigned long long blocks = static_cast<unsigned long long>(r.blocks_per_batch) * a.batch;
     if (p.states == kReorderStates || grid + blocks > 0x7FFFFFFFull) {
       const cudaError_t err = launch_some(p, static_cast<unsigned int>(grid), static_cast<cudaStream_t>(a.stream));

@@ -11,7 +11,7 @@
 // 2^106 where it meets a 16 q u; a 32-bit X as three such columns of 8 bits each, which sum up to it exactly.  A binary16 X is
 // staged as it is (a sixteenth of its smallest numbers could not be written) and the products with 16 q u are summed apart.
 // Infinities and NaN, and numbers from 2^18 on in the wide types, make every output of their row infinite or NaN: outputs
-// that are get computed once more as the formula has it.  At the other end the products end at 2^-126.
+// that are get computed once more as the formula has it.  At the other end the sums of x q end at 2^-103 (2^-126 in units of 2^-23).
 //
 // Zero points leave the products:  sum x (q - z) = sum x q - z sum x,  the sums of x by groups taken once per block, in 32
 // bits, where the accumulators start.  That costs the rounding of sum x q, about twice that of the result, and saves a
@@ -42,11 +42,8 @@ constexpr int kQ4Pitch = kQ4Step / 2 + 4;     // bytes between rows of a stage t
 template <bool TMA> constexpr int kQ4Stage = kQ4Rows * (TMA ? kQ4Step / 2 : kQ4Pitch);
 constexpr int kQ4Stages = 2;                  // of a warp; three measured slower (128000 x 4096 read alone: 53 us instead of 45)
 constexpr int kQ4MaxSlices = 4;               // blocks of a cluster that share k
-// Warps of a block: 16, or 8 where the sums of more than eight columns take the registers or X the shared memory.
 constexpr int kQ4SumStride = kQ4Rows + 4;     // floats between columns of a warp's sums: no bank twice
 template <int NT> constexpr int kQ4Buffer = NT * 8 * kQ4SumStride; // floats of a warp's sums
-// X is read eight columns at a time: what lies behind a panel's last word has to be there.
-template <int NT> constexpr int kQ4Overread = NT * 8 * 64;
 
 struct Q4Params {
   const void* X; long long ldx;
@@ -326,7 +323,8 @@ __device__ __forceinline__ void worker_barrier(int worker, int warps) {
   asm volatile("bar.sync %0, %1;" ::"r"(worker + 1), "r"(warps * 32) : "memory");
 }
 
-// NT tiles of eight columns of X.
+// NT tiles of eight columns of X.  WARPS: 16, or 8 where the sums of more than eight columns take the registers or X the shared
+// memory.
 template <bool BF16, int NT, int WARPS, int LW, bool TMA, bool ZEROS>
 __global__ void __launch_bounds__(32 * WARPS, 1)
 q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Params p) {

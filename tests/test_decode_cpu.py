@@ -66,6 +66,17 @@ def test_q4_types_and_groups():
     assert _lib.load().cuasr_b200_q4_product(None) == Status.kErrorInvalidProblem
 
 
+@pytest.mark.parametrize("change,status", [
+    ({"n": 2 ** 31 - 2 ** 17, "ldy": 2 ** 31}, Status.kSuccess), ({"n": 2 ** 31 - 1, "ldy": 2 ** 31}, Status.kErrorNotSupported),
+    ({"k": 2 ** 31 - 2 ** 17, "ldx": 2 ** 31, "ldw": 2 ** 30, "lds": 2 ** 26}, Status.kSuccess),
+    ({"k": 2 ** 31 - 1, "ldx": 2 ** 31, "ldw": 2 ** 30, "lds": 2 ** 26}, Status.kErrorNotSupported),
+    ({"m": 32 * 65535}, Status.kSuccess), ({"m": 32 * 65535 + 1}, Status.kErrorNotSupported),
+    ({"lds": 2 ** 40, "z": (P, 2 ** 40)}, Status.kSuccess),
+])
+def test_q4_limits(change, status):
+    assert Q4Product(DType.F16, group=32).can_implement(q4_args(**change)) == status
+
+
 def test_semiring_products_take_no_16_bit_types():
     for dtype in (DType.F16, DType.BF16):
         with pytest.raises(ValueError):
@@ -167,6 +178,12 @@ FAR = P + (1 << 30)
     ([view(src=P + 128 * i) for i in range(256)], {}, Status.kSuccess),
     ([view(src=P + 128 * i) for i in range(257)], {}, Status.kErrorNotSupported),
     ([view(strides=(1 << 62, 16, 8, 4))], {}, Status.kErrorInvalidProblem),
+    # in place, the rows of one search that are only read are those of another that are written
+    ([view(strides=(32, 16, 8, 4))], {"keep": 2}, Status.kErrorInvalidProblem),
+    ([view(dst=FAR, strides=(32, 16, 8, 4), dst_strides=(32, 16, 8, 4))], {"keep": 2}, Status.kSuccess),
+    # more columns than a grid has blocks for
+    ([view(src=P + 1, strides=(1 << 42, 1 << 40, 1 << 40, 1), nbytes=1 << 40, segments=1, positions=1)], {}, Status.kErrorNotSupported),
+    ([view(src=P, strides=(1 << 42, 1 << 40, 1 << 40, 1), nbytes=1 << 40, segments=1, positions=1)], {"batch": 1}, Status.kSuccess),
 ])
 def test_reorder_refusals(states, change, status):
     op = ReorderStates()

@@ -120,6 +120,67 @@ def test_q4_same_bits_every_time(cuda_device):
     done()
 
 
+# Sizes at which the rows of weights and k are shared out in different ways: several warps to 32 rows, several blocks to k, an X
+# that shared memory holds in part only, and each of them with weight rows on 16-byte boundaries and off them.
+SHARED_OUT = [(1, 40, 70000, 128, DType.BF16), (1, 5000, 300, 64, DType.F16), (2, 4000, 4000, 32, DType.BF16), (3, 30000, 700, 64, DType.F32),
+              (5, 64, 33000, 32, DType.F16), (8, 3000, 9000, 128, DType.F16), (10, 100, 9001, 64, DType.F32), (12, 9000, 2500, 128, DType.BF16),
+              (16, 600, 14000, 64, DType.F16), (20, 17, 2049, 32, DType.BF16), (32, 64, 20000, 128, DType.BF16), (32, 5000, 4100, 128, DType.F16)]
+
+
+@pytest.mark.parametrize("m,n,k,group,x", SHARED_OUT)
+@pytest.mark.parametrize("byte_offset", [0, 1])
+def test_q4_shared_out(cuda_device, m, n, k, group, x, byte_offset):
+    Q4Case(m, n, k, group, x, DType.F32, zeros=byte_offset == 0, pad=(-(k + 1) // 2) % 16, byte_offset=byte_offset, seed=k).check()
+
+
+@pytest.mark.parametrize("m,n,k,group,x", [c for c in SHARED_OUT if c[0] >= 3])
+def test_q4_infinities_in_one_row(cuda_device, m, n, k, group, x):
+    """An infinity, a NaN and numbers that the products do not hold, in a row each; outputs that 32 bits do not hold."""
+    c = Q4Case(m, n, k, group, x, DType.F32, pad=3, seed=k)
+    c.X[0, k - 1], c.X[1, 0] = -INF, math.nan
+    if x != DType.F16:
+        c.X[2, ::7] = 2.0 ** 40
+        c.X[2, 1] = 2.0 ** 120
+    y, w = c.run().clone(), c.weights()
+    done()
+    want = c.X[:, :k].double() @ w.T
+    assert torch.isnan(y[1]).all() and torch.equal(torch.isnan(y[0]), w[:, k - 1] == 0)
+    ruled = w[:, k - 1] != 0
+    assert torch.equal(y[0][ruled], torch.where(w[:, k - 1] > 0, -INF, INF).float()[ruled])
+    # as in Q4Case.check
+    steps = min(group, k) + -(-k // group) + 16
+    bound = steps * 2.0 ** -23 * (c.X[2:, :k].double().abs() @ w.abs().T) + 2.0 ** -24 * 1.001 * want[2:].abs()
+    assert ((y[2:].double() - want[2:]).abs() <= bound).all()
+
+
+def test_q4_results_beyond_a_type(cuda_device):
+    """Results that 16 bits do not hold become infinite, those of all zeros are zero."""
+    c = Q4Case(3, 100, 256, 64, DType.BF16, DType.F16)
+    c.X[0] = 2.0 ** 17
+    c.X[1] = 0
+    c.W.fill_(0xFF)
+    y = c.run()
+    done()
+    assert (y[0] == INF).all() and (y[1] == 0).all() and torch.isfinite(y[2]).all()
+
+
+def test_q4_overlapping_calls_on_one_x(cuda_device):
+    """Calls that share X and the weights, on two streams, each with its own Y."""
+    first = Q4Case(4, 6000, 2048, 128, DType.BF16, DType.F32)
+    want = first.run().clone()
+    torch.cuda.synchronize()
+    others = [Q4Case(4, 6000, 2048, 128, DType.BF16, DType.F32) for _ in range(2)]
+    for c in others:
+        c.X, c.W, c.scales = first.X, first.W, first.scales
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in others]
+    for _ in range(4):
+        for c, s in zip(others, streams):
+            c.run(s)
+    done()
+    assert all(torch.equal(c.Y, want) for c in others)
+
+
 # ---- beam steps -----------------------------------------------------------------------------------------------------
 def plain_step(logits, scores, keep, normalise, finished, end_token):
     """Values, parents and tokens of every search on the host, sorted as documented; also a function that gives the value of
@@ -302,6 +363,28 @@ def test_beam_step_first_step_and_scores_in_place(cuda_device):
     assert all(e[1] == 0 for s in got for e in s)
 
 
+@pytest.mark.parametrize("dtype", REALS)
+@pytest.mark.parametrize("vocab", [4000, 131071])
+@pytest.mark.parametrize("keep", [1, 33, 64])
+def test_beam_step_runs_of_equal_logits(cuda_device, dtype, vocab, keep):
+    """Plateaus that rise along the vocabulary, each wider than a warp's room for candidates, and one that begins inside another
+    tile than it ends; equal values between prefixes too."""
+    steps = torch.arange(vocab, device="cuda") // 700
+    logits = torch.stack((steps, steps.flip(0), steps % 3)).float().to(TORCH[dtype])[None].contiguous()
+    check_step(logits, torch.zeros(1, 3, device="cuda"), keep, normalise=False)
+
+
+@pytest.mark.parametrize("normalise", [False, True])
+@pytest.mark.parametrize("beams,keep", [(257, 4), (1024, 8), (130, 64), (512, 17)])
+def test_beam_step_many_prefixes(cuda_device, normalise, beams, keep):
+    g = gen(beams)
+    logits = torch.randint(-3, 4, (2, beams, 50), generator=g, device="cuda").float()
+    finished = (torch.rand(2, beams, generator=g, device="cuda") < 0.3).to(torch.uint8)
+    scores = -torch.randint(0, 3, (2, beams), generator=g, device="cuda").float()
+    scores[1, ::2] = -INF
+    check_step(logits + torch.rand(2, beams, 50, generator=g, device="cuda") * normalise, scores, keep, normalise, finished)
+
+
 def test_beam_step_logits_beyond_32_bit_offsets(cuda_device):
     """Element offsets above 2^31: two searches whose rows lie 2^31 + 16 half-precision numbers apart."""
     far = 2 ** 31 + 16
@@ -410,6 +493,13 @@ def test_reorder_does_not_follow_parents_out_of_range(cuda_device):
     x = torch.randn(2, 3, 100, generator=gen(9), device="cuda")
     check_reorder([x], torch.tensor([[2, 3, 0], [0, 2 ** 31 - 1, -2 ** 31]], device="cuda", dtype=torch.int32))
     assert device_status() == 4 and device_status() == 0
+
+
+def test_reorder_ignores_lengths_out_of_range(cuda_device):
+    x = torch.randn(3, 4, 2, 11, 8, generator=gen(31), device="cuda")
+    lengths = torch.tensor([-5, 2 ** 31 - 1, 0], device="cuda", dtype=torch.int32)
+    check_reorder([x], parents_of(3, 4, 4, 32), lengths=lengths, position_dim=3)
+    done()
 
 
 def test_reorder_beyond_32_bit_offsets(cuda_device):
