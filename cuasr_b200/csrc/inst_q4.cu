@@ -26,12 +26,14 @@ void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
   plan->smem = fixed - 16 + plan->xsum_bytes + panel * 512 * s.columns + all_stages;
 }
 
-Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, int sms) {
+// clusters[i]: clusters of 2^i blocks that the device runs at a time.
+Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, const int (&clusters)[kQ4SliceChoices]) {
   Q4Plan best;
   double best_cost = 0;
   for (int warps = shape.column_tiles == 1 ? 16 : 8; warps >= 8; warps /= 2)
     for (int parts = 1; parts <= 8; parts *= 2)
-      for (int s = 1; s <= kQ4MaxSlices && (s == 1 || s <= steps); s *= 2) {
+      for (int i = 0; i < kQ4SliceChoices && (i == 0 || 1 << i <= steps); ++i) {
+        const int s = 1 << i;
         Q4Plan plan;
         plan.warps = warps;
         plan.parts = parts;
@@ -39,7 +41,7 @@ Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, int sms) 
         const int workers = warps / parts, slice_steps = (steps + s - 1) / s;
         fit(&plan, slice_steps, shape);
         if (plan.panel_steps <= 0) continue;
-        const int blocks = std::max(1, std::min((units + workers - 1) / workers, std::max(1, sms / s)));
+        const int blocks = std::max(1, std::min((units + workers - 1) / workers, clusters[i]));
         const double rounds = static_cast<double>(((units + workers - 1) / workers + blocks - 1) / blocks) * passes;
         // In microseconds, from measurements between 1024 x 1024 and 128000 x 4096: a warp's step with all warps at it 1.7 (16 of
         // them; 1.4 with eight, 2 for 32 columns), a worker's sums 1.3, a cluster's 2 more; X laid out by a block 0.5 for a step of
@@ -57,6 +59,27 @@ Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, int sms) 
         }
       }
   return best;
+}
+
+// A cluster lies within one of the device's groups of SMs, whose sizes its multiple need not divide: of 148 SMs 132 are in
+// clusters of four at a time.  One cluster more than that runs behind all others (128000 x 4096, 32 rows: 380 us with 37).
+cudaError_t count_clusters(int (&clusters)[kQ4SliceChoices], int sms) {
+  static std::atomic<uint64_t> known[64];          // by device: 16 bits for each size
+  static_assert(kQ4SliceChoices <= 4, "16 bits each");
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  uint64_t packed = known[dev & 63].load(std::memory_order_relaxed);
+  if (packed == 0) {
+    for (int i = 0; i < kQ4SliceChoices; ++i) {
+      int n = sms;
+      if (i > 0 && (err = q4_active_clusters(1 << i, &n)) != cudaSuccess) return err;
+      packed |= static_cast<uint64_t>(std::max(1, std::min(n, 0xFFFF))) << (16 * i);
+    }
+    known[dev & 63].store(packed, std::memory_order_relaxed);
+  }
+  for (int i = 0; i < kQ4SliceChoices; ++i) clusters[i] = static_cast<int>(packed >> (16 * i) & 0xFFFF);
+  return cudaSuccess;
 }
 
 // Weight rows as bytes: boxes of 32 rows by the 64 bytes of half a step; zeros outside.
@@ -109,14 +132,17 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
   const bool tma = weight_map(&map, a);
   const Q4Shape shape = {columns, nt, 8 / lw, tma ? kQ4Stage<true> : kQ4Stage<false>};
   p.units = (a.n - 1) / kQ4Rows + 1;
-  const Q4Plan plan = plan_q4(p.units, steps, passes, shape, dev.sms);
+  int clusters[kQ4SliceChoices];
+  cudaError_t err = count_clusters(clusters, dev.sms);
+  if (err != cudaSuccess) return err;
+  const Q4Plan plan = plan_q4(p.units, steps, passes, shape, clusters);
   if (plan.smem == 0) return cudaErrorInvalidValue;      // no launch fits: never for one block per SM and one slice
   p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
   const Q4Launch l = {plan.grid, passes, plan.smem, static_cast<cudaStream_t>(a.stream)};
-  const cudaError_t err = nt == 4          ? launch_q4_columns<4, 8>(lw, tma, map, p, l)
-                          : nt == 2          ? launch_q4_columns<2, 8>(lw, tma, map, p, l)
-                          : plan.warps == 16 ? launch_q4_columns<1, 16>(lw, tma, map, p, l)
-                                             : launch_q4_columns<1, 8>(lw, tma, map, p, l);
+  err = nt == 4            ? launch_q4_columns<4, 8>(lw, tma, map, p, l)
+        : nt == 2          ? launch_q4_columns<2, 8>(lw, tma, map, p, l)
+        : plan.warps == 16 ? launch_q4_columns<1, 16>(lw, tma, map, p, l)
+                           : launch_q4_columns<1, 8>(lw, tma, map, p, l);
   if (err == cudaSuccess) ++*launches;
   return err;
 }

@@ -36,6 +36,9 @@ cudaError_t launch_q4_kernel(const CUtensorMap& map, const Q4Params& p, const Q4
   return cudaLaunchKernelEx(&config, kernel, map, p);
 }
 
+// Clusters of `slices` blocks, each with an SM to itself, that the device runs at a time (inst_q4_1_16.cu).
+cudaError_t q4_active_clusters(int slices, int* clusters);
+
 template <int NT, int WARPS>
 cudaError_t launch_q4_columns(int lw, bool tma, const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
   const bool zeros = p.zeros != nullptr, bf16 = p.type_x != CUASR_F16;

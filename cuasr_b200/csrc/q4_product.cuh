@@ -41,7 +41,7 @@ constexpr int kQ4Step = 256;                  // k of a step, two halves of 16 w
 constexpr int kQ4Pitch = kQ4Step / 2 + 4;     // bytes between rows of a stage that the lanes fill: one more aligned word
 template <bool TMA> constexpr int kQ4Stage = kQ4Rows * (TMA ? kQ4Step / 2 : kQ4Pitch);
 constexpr int kQ4Stages = 2;                  // of a warp; three measured slower (128000 x 4096 read alone: 53 us instead of 45)
-constexpr int kQ4MaxSlices = 4;               // blocks of a cluster that share k
+constexpr int kQ4SliceChoices = 3;            // 1, 2 or 4 blocks of a cluster share k
 constexpr int kQ4SumStride = kQ4Rows + 4;     // floats between columns of a warp's sums: no bank twice
 template <int NT> constexpr int kQ4Buffer = NT * 8 * kQ4SumStride; // floats of a warp's sums
 
