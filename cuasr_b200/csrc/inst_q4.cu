@@ -11,12 +11,12 @@ struct Q4Plan {
 };
 // What the shape of X and of the groups makes of a block.
 struct Q4Shape {
-  int columns, column_tiles, groups_per_step, stage_bytes;
+  int columns, column_tiles, rows, groups_per_step, stage_bytes;      // rows: weight rows of a worker
 };
 
 // Shared memory of a block: stages, sums, X of a panel and what is read behind it (X is read eight columns at a time).
 void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
-  plan->sum_bytes = plan->warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * kQ4SumStride * 4;
+  plan->sum_bytes = plan->warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * (s.rows + kQ4SumPad) * 4;
   const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = kQ4Stages * plan->warps * s.stage_bytes;
   const int per_step = 512 * s.columns + 4 * s.groups_per_step * ((s.columns + 1) / 2 * 2), room = kQ4SmemPerBlock - fixed;
   int panel = slice_steps;
@@ -30,7 +30,7 @@ void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
 Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, const int (&clusters)[kQ4SliceChoices]) {
   Q4Plan best;
   double best_cost = 0;
-  for (int warps = shape.column_tiles == 1 ? 16 : 8; warps >= 8; warps /= 2)
+  for (int warps = 16; warps >= (shape.column_tiles == 1 ? 8 : 16); warps /= 2)
     for (int parts = 1; parts <= 8; parts *= 2)
       for (int i = 0; i < kQ4SliceChoices && (i == 0 || 1 << i <= steps); ++i) {
         const int s = 1 << i;
@@ -82,8 +82,8 @@ cudaError_t count_clusters(int (&clusters)[kQ4SliceChoices], int sms) {
   return cudaSuccess;
 }
 
-// Weight rows as bytes: boxes of 32 rows by the 64 bytes of half a step; zeros outside.
-bool weight_map(CUtensorMap* map, const cuasr_b200_q4_args_t& a) {
+// Weight rows as bytes: boxes of a worker's rows by the 64 bytes of half a step; zeros outside.
+bool weight_map(CUtensorMap* map, const cuasr_b200_q4_args_t& a, int rows) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static const Encode encode = [] {
@@ -95,7 +95,7 @@ bool weight_map(CUtensorMap* map, const cuasr_b200_q4_args_t& a) {
   if (encode == nullptr || reinterpret_cast<uintptr_t>(a.W) % 16 != 0 || a.ldw % 16 != 0 || a.ldw >= (1LL << 40)) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>((static_cast<int64_t>(a.k) + 1) / 2), static_cast<cuuint64_t>(a.n)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.ldw)};
-  const cuuint32_t box[2] = {kQ4Step / 4, kQ4Rows}, ones[2] = {1, 1};
+  const cuuint32_t box[2] = {kQ4Step / 4, static_cast<cuuint32_t>(rows)}, ones[2] = {1, 1};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(a.W), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -129,9 +129,10 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
   const int lw = a.group % 128 == 0 || a.group >= a.k ? 4 : a.group % 64 == 0 ? 2 : 1;
   const int steps = (a.k + kQ4Step - 1) / kQ4Step;
   CUtensorMap map = {};
-  const bool tma = weight_map(&map, a);
-  const Q4Shape shape = {columns, nt, 8 / lw, tma ? kQ4Stage<true> : kQ4Stage<false>};
-  p.units = (a.n - 1) / kQ4Rows + 1;
+  const int tiles = nt == 1 ? 2 : 1;
+  const bool tma = weight_map(&map, a, 16 * tiles);
+  const Q4Shape shape = {columns, nt, 16 * tiles, 8 / lw, (tma ? kQ4Stage<true, 1> : kQ4Stage<false, 1>) * tiles};
+  p.units = (a.n - 1) / shape.rows + 1;
   int clusters[kQ4SliceChoices];
   cudaError_t err = count_clusters(clusters, dev.sms);
   if (err != cudaSuccess) return err;
@@ -139,10 +140,10 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
   if (plan.smem == 0) return cudaErrorInvalidValue;      // no launch fits: never for one block per SM and one slice
   p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
   const Q4Launch l = {plan.grid, passes, plan.smem, static_cast<cudaStream_t>(a.stream)};
-  err = nt == 4            ? launch_q4_columns<4, 8>(lw, tma, map, p, l)
-        : nt == 2          ? launch_q4_columns<2, 8>(lw, tma, map, p, l)
-        : plan.warps == 16 ? launch_q4_columns<1, 16>(lw, tma, map, p, l)
-                           : launch_q4_columns<1, 8>(lw, tma, map, p, l);
+  err = nt == 4            ? launch_q4_columns<4, 1, 16>(lw, tma, map, p, l)
+        : nt == 2          ? launch_q4_columns<2, 1, 16>(lw, tma, map, p, l)
+        : plan.warps == 16 ? launch_q4_columns<1, 2, 16>(lw, tma, map, p, l)
+                           : launch_q4_columns<1, 2, 8>(lw, tma, map, p, l);
   if (err == cudaSuccess) ++*launches;
   return err;
 }

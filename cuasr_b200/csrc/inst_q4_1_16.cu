@@ -1,11 +1,11 @@
 // Products with 4-bit weights, 8 columns at a time, 16 warps to a block.
 #include "q4_launch.cuh"
 namespace cuasr_b200 {
-template cudaError_t launch_q4_columns<1, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+template cudaError_t launch_q4_columns<1, 2, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
 
 cudaError_t q4_active_clusters(int slices, int* clusters) {
   static std::atomic<uint64_t> allowed{0};
-  auto kernel = q4_kernel<true, 1, 16, 4, true, false>;
+  auto kernel = q4_kernel<true, 1, 2, 16, 4, true, false>;
   cudaError_t err = allow_shared_memory(reinterpret_cast<const void*>(kernel), kQ4SmemPerBlock, allowed);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config = {};

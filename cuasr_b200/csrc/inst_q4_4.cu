@@ -1,5 +1,5 @@
 // Products with 4-bit weights, 32 columns at a time, 8 warps to a block.
 #include "q4_launch.cuh"
 namespace cuasr_b200 {
-template cudaError_t launch_q4_columns<4, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+template cudaError_t launch_q4_columns<4, 1, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
 }  // namespace cuasr_b200

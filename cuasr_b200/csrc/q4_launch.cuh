@@ -14,10 +14,10 @@ struct Q4Launch {
   cudaStream_t stream;
 };
 
-template <bool BF16, int NT, int WARPS, int LW, bool TMA, bool ZEROS>
+template <bool BF16, int NT, int RT, int WARPS, int LW, bool TMA, bool ZEROS>
 cudaError_t launch_q4_kernel(const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
   static std::atomic<uint64_t> allowed{0};
-  auto kernel = q4_kernel<BF16, NT, WARPS, LW, TMA, ZEROS>;
+  auto kernel = q4_kernel<BF16, NT, RT, WARPS, LW, TMA, ZEROS>;
   const cudaError_t err = allow_shared_memory(reinterpret_cast<const void*>(kernel), kQ4SmemPerBlock, allowed);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config = {};
@@ -39,12 +39,12 @@ cudaError_t launch_q4_kernel(const CUtensorMap& map, const Q4Params& p, const Q4
 // Clusters of `slices` blocks, each with an SM to itself, that the device runs at a time (inst_q4_1_16.cu).
 cudaError_t q4_active_clusters(int slices, int* clusters);
 
-template <int NT, int WARPS>
+template <int NT, int RT, int WARPS>
 cudaError_t launch_q4_columns(int lw, bool tma, const CUtensorMap& map, const Q4Params& p, const Q4Launch& l) {
   const bool zeros = p.zeros != nullptr, bf16 = p.type_x != CUASR_F16;
 #define Q4_CASE(L, V, Z)                                                            \
   if (lw == L && tma == V && zeros == Z)                                            \
-    return bf16 ? launch_q4_kernel<true, NT, WARPS, L, V, Z>(map, p, l) : launch_q4_kernel<false, NT, WARPS, L, V, Z>(map, p, l);
+    return bf16 ? launch_q4_kernel<true, NT, RT, WARPS, L, V, Z>(map, p, l) : launch_q4_kernel<false, NT, RT, WARPS, L, V, Z>(map, p, l);
 #define Q4_CASES(L) Q4_CASE(L, false, false) Q4_CASE(L, true, false) Q4_CASE(L, false, true) Q4_CASE(L, true, true)
   Q4_CASES(1) Q4_CASES(2) Q4_CASES(4)
 #undef Q4_CASES
@@ -52,9 +52,9 @@ cudaError_t launch_q4_columns(int lw, bool tma, const CUtensorMap& map, const Q4
   return cudaErrorInvalidValue;
 }
 
-extern template cudaError_t launch_q4_columns<1, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
-extern template cudaError_t launch_q4_columns<1, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
-extern template cudaError_t launch_q4_columns<2, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
-extern template cudaError_t launch_q4_columns<4, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<1, 2, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<1, 2, 8>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<2, 1, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
+extern template cudaError_t launch_q4_columns<4, 1, 16>(int, bool, const CUtensorMap&, const Q4Params&, const Q4Launch&);
 
 }  // namespace cuasr_b200

@@ -36,14 +36,13 @@
 
 namespace cuasr_b200 {
 
-constexpr int kQ4Rows = 32;                   // weight rows of a worker: two tiles of the instruction
 constexpr int kQ4Step = 256;                  // k of a step, two halves of 16 words of a weight row, 4 of them to a lane
 constexpr int kQ4Pitch = kQ4Step / 2 + 4;     // bytes between rows of a stage that the lanes fill: one more aligned word
-template <bool TMA> constexpr int kQ4Stage = kQ4Rows * (TMA ? kQ4Step / 2 : kQ4Pitch);
+// Weight rows of a worker are RT tiles of the instruction.
+template <bool TMA, int RT> constexpr int kQ4Stage = 16 * RT * (TMA ? kQ4Step / 2 : kQ4Pitch);
 constexpr int kQ4Stages = 2;                  // of a warp; three measured slower (128000 x 4096 read alone: 53 us instead of 45)
 constexpr int kQ4SliceChoices = 3;            // 1, 2 or 4 blocks of a cluster share k
-constexpr int kQ4SumStride = kQ4Rows + 4;     // floats between columns of a warp's sums: no bank twice
-template <int NT> constexpr int kQ4Buffer = NT * 8 * kQ4SumStride; // floats of a warp's sums
+constexpr int kQ4SumPad = 4;                  // floats between columns of a warp's sums, besides its rows: no bank twice
 
 struct Q4Params {
   const void* X; long long ldx;
@@ -54,7 +53,7 @@ struct Q4Params {
   int m, n, k, group, groups, group_shift;    // group_shift: log2(group), or -1
   int type_x, type_y, type_scale;             // cuasr_dtype_t
   int rows;                                   // rows of X of a pass (blockIdx.y)
-  int units, parts, slices;                   // 32 weight rows each; warps of a worker; blocks that share k
+  int units, parts, slices;                   // 16 RT weight rows each; warps of a worker; blocks that share k
   int panel_steps;                            // steps whose X fits into shared memory; a multiple of parts if not all
   int sum_bytes, xsum_bytes;
   unsigned int* status;
@@ -161,26 +160,29 @@ __device__ __forceinline__ void copy_word(const Q4Params& p, unsigned char* stag
     *reinterpret_cast<uint32_t*>(to) = v;
   }
 }
+template <int RT>
 __device__ __forceinline__ void copy_step(const Q4Params& p, unsigned char* stage, long long first_row, int step, int lane, int row_bytes,
                                           const unsigned char* last) {
   const unsigned char* q = p.W + first_row * p.ldw + static_cast<long long>(step) * (kQ4Step / 2);
-  if (first_row + kQ4Rows <= p.n && q - 3 >= p.W && q + (kQ4Rows - 1) * p.ldw + kQ4Step / 2 + 4 <= last) {
+  constexpr int kRows = 16 * RT;
+  if (first_row + kRows <= p.n && q - 3 >= p.W && q + (kRows - 1) * p.ldw + kQ4Step / 2 + 4 <= last) {
     // every word lies inside the operand; what lies behind a row's end meets zeros of X
     const uint32_t to = smem_u32(stage) + lane * 4;
 #pragma unroll 8
-    for (int r = 0; r < kQ4Rows; ++r) {
+    for (int r = 0; r < kRows; ++r) {
       const unsigned char* a = q - (reinterpret_cast<uintptr_t>(q) & 3) + lane * 4;
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + r * kQ4Pitch), "l"(a) : "memory");
       q += p.ldw;
     }
+    if (lane >= kRows) return;
     const unsigned char* mine = p.W + (first_row + lane) * p.ldw + static_cast<long long>(step) * (kQ4Step / 2);
     const unsigned char* a = mine - (reinterpret_cast<uintptr_t>(mine) & 3) + 128;
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(stage) + lane * kQ4Pitch + 128), "l"(a) : "memory");
     return;
   }
 #pragma unroll 1
-  for (int r = 0; r < kQ4Rows; ++r) copy_word(p, stage, first_row + r, step, r, lane, row_bytes, last);
-  copy_word(p, stage, first_row + lane, step, lane, 32, row_bytes, last);
+  for (int r = 0; r < kRows; ++r) copy_word(p, stage, first_row + r, step, r, lane, row_bytes, last);
+  if (lane < kRows) copy_word(p, stage, first_row + lane, step, lane, 32, row_bytes, last);
 }
 
 // Eight values of a row of X from k on, zeros from p.k on: E = uint32_t for 32-bit rows, unsigned short for 16-bit ones.
@@ -325,19 +327,19 @@ __device__ __forceinline__ void worker_barrier(int worker, int warps) {
 
 // NT tiles of eight columns of X.  WARPS: 16, or 8 where the sums of more than eight columns take the registers or X the shared
 // memory.
-template <bool BF16, int NT, int WARPS, int LW, bool TMA, bool ZEROS>
+template <bool BF16, int NT, int RT, int WARPS, int LW, bool TMA, bool ZEROS>
 __global__ void __launch_bounds__(32 * WARPS, 1)
 q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Params p) {
   extern __shared__ __align__(1024) unsigned char q4_smem[];
-  constexpr int kThreads = 32 * WARPS, RT = kQ4Rows / 16;
+  constexpr int kThreads = 32 * WARPS, kRows = 16 * RT, kStage = kQ4Stage<TMA, RT>, kSumStride = kRows + kQ4SumPad, kBuffer = NT * 8 * kSumStride;
   __shared__ uint64_t full[WARPS][kQ4Stages];
   __shared__ unsigned int abandoned;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int parts = p.parts, part_of = warp % parts, local = warp / parts, workers_here = WARPS / parts;
-  unsigned char* stages = q4_smem + warp * kQ4Stages * kQ4Stage<TMA>;
-  float* all_sums = reinterpret_cast<float*>(q4_smem + WARPS * kQ4Stages * kQ4Stage<TMA>);
+  unsigned char* stages = q4_smem + warp * kQ4Stages * kStage;
+  float* all_sums = reinterpret_cast<float*>(q4_smem + WARPS * kQ4Stages * kStage);
   const int buffers = max(parts - 1, 1);                   // of a worker
-  float* sums = all_sums + local * buffers * kQ4Buffer<NT>;
+  float* sums = all_sums + local * buffers * kBuffer;
   float* xsums = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(all_sums) + p.sum_bytes);
   uint4* xs = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(xsums) + p.xsum_bytes);
   const int slice = p.slices > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -368,15 +370,15 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
   const int row_bytes = (p.k + 1) / 2;
   auto copy_ahead = [&] {           // TMA: lane 0 alone
     if (ahead_unit < p.units) {
-      unsigned char* to = stages + ahead_stage * kQ4Stage<TMA>;
+      unsigned char* to = stages + ahead_stage * kStage;
       if constexpr (TMA) {
         uint64_t* bar = &full[warp][ahead_stage];
-        const int y = ahead_unit * kQ4Rows, x = ahead * (kQ4Step / 2);
-        mbar_arrive_expect_tx(bar, kQ4Stage<TMA>);
+        const int y = ahead_unit * kRows, x = ahead * (kQ4Step / 2);
+        mbar_arrive_expect_tx(bar, kStage);
         tma_load_2d(to, &map, bar, x, y);
-        tma_load_2d(to + kQ4Stage<TMA> / 2, &map, bar, x + kQ4Step / 4, y);
+        tma_load_2d(to + kStage / 2, &map, bar, x + kQ4Step / 4, y);
       } else {
-        copy_step(p, to, static_cast<long long>(ahead_unit) * kQ4Rows, ahead, lane, row_bytes, p.W + (p.n - 1) * p.ldw + row_bytes);
+        copy_step<RT>(p, to, static_cast<long long>(ahead_unit) * kRows, ahead, lane, row_bytes, p.W + (p.n - 1) * p.ldw + row_bytes);
       }
       ahead += parts;
       if (ahead >= end) { ahead = begin + part_of; ahead_unit += workers; }
@@ -388,8 +390,8 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
     for (int s = 0; s < (TMA ? kQ4Stages : kQ4Stages - 1); ++s) copy_ahead();
 
   // Scales and zero points of a step, loaded one step ahead, for both its halves.  Where half a step has one group, lane
-  // (g, t) has those of row t * 8 + g; else those of its t-th group for rows g, 8 + g, ...
-  constexpr int kMine = LW == 4 ? 1 : 4;
+  // (g, t) has those of row t * 8 + g (of two tiles; of one, t and t + 2 have the same); else those of its t-th group for rows g, 8 + g, ...
+  constexpr int kMine = LW == 4 ? 1 : 2 * RT;
   uint32_t next_scale[2][kMine], next_zero[2][kMine];
   const int scale_shift = p.type_scale == CUASR_BF16 ? 16 : 0;
   auto load_scales = [&](int unit, int step) {
@@ -403,7 +405,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
     }
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
-      const long long row = min(unit * kQ4Rows + (LW == 4 ? t : j) * 8 + g, p.n - 1);      // rows behind the last get the last one's
+      const long long row = min(unit * kRows + (LW == 4 ? t % (2 * RT) : j) * 8 + g, p.n - 1);      // rows behind the last get the last one's
       const long long at = row * p.ld_scales;
       if (p.type_scale == CUASR_F32) {
 #pragma unroll
@@ -430,7 +432,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
     if constexpr (!TMA) {
 #pragma unroll
       for (int j = 0; j < 2 * RT; ++j)
-        shift[j] = static_cast<unsigned int>((reinterpret_cast<uintptr_t>(p.W) + (static_cast<long long>(unit) * kQ4Rows + j * 8 + g) * p.ldw) & 3) * 8;
+        shift[j] = static_cast<unsigned int>((reinterpret_cast<uintptr_t>(p.W) + (static_cast<long long>(unit) * kRows + j * 8 + g) * p.ldw) & 3) * 8;
     }
     float acc[RT][NT][4] = {};
     for (int panel = begin; panel < end; panel += p.panel_steps) {
@@ -467,7 +469,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const unsigned char* words = stages + stage * kQ4Stage<TMA> + (TMA ? u * kQ4Stage<TMA> / 2 : u * kQ4Step / 4);
+          const unsigned char* words = stages + stage * kStage + (TMA ? u * kStage / 2 : u * kQ4Step / 4);
           const uint4* x = xs + (((step - panel) * 2 + u) * 16 * columns + lane);
           uint32_t w[2 * RT][4];
 #pragma unroll
@@ -532,40 +534,41 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
     }
 
     // All but one warp of the worker put their sums down; that one, another every time, adds them to its own.
-    const int first_row = unit * kQ4Rows, last_row = min(kQ4Rows, p.n - first_row) - 1;
+    const int first_row = unit * kRows, last_row = min(kRows, p.n - first_row) - 1;
     auto each_sum = [&](auto&& f) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) f((nt * 8 + t * 2 + c % 2) * kQ4SumStride + rt * 16 + c / 2 * 8 + g, acc[rt][nt][c]);
+          for (int c = 0; c < 4; ++c) f((nt * 8 + t * 2 + c % 2) * kSumStride + rt * 16 + c / 2 * 8 + g, acc[rt][nt][c]);
     };
     const int adder = round % parts;
     if (mine) {
       if (parts > 1) {
         worker_barrier(local, parts);      // the sums before have been read
         if (part_of != adder) {
-          float* to = sums + (part_of < adder ? part_of : part_of - 1) * kQ4Buffer<NT>;
+          float* to = sums + (part_of < adder ? part_of : part_of - 1) * kBuffer;
           each_sum([&](int at, float v) { to[at] = v; });
         }
         worker_barrier(local, parts);
       }
       if (part_of == adder) {
-        for (int v = 0; v < parts - 1; ++v) each_sum([&](int at, float& a) { a += sums[v * kQ4Buffer<NT> + at]; });
+        for (int v = 0; v < parts - 1; ++v) each_sum([&](int at, float& a) { a += sums[v * kBuffer + at]; });
         each_sum([&](int at, float v) { sums[at] = v; });
       }
       if (p.slices == 1) {
         // the rows of X are shared out among the warps
         if (parts > 1) worker_barrier(local, parts);
         else __syncwarp();
-        if (lane <= last_row)
-          for (int r = part_of; r < rows; r += parts) {
-            float s = sums[r * kQ4SumStride + lane];
-            if (columns != rows) s += sums[(r + rows) * kQ4SumStride + lane] + sums[(r + 2 * rows) * kQ4SumStride + lane];
+        const int j = lane % kRows;
+        if (j <= last_row)
+          for (int r = part_of * (2 / RT) + lane / kRows; r < rows; r += parts * (2 / RT)) {
+            float s = sums[r * kSumStride + j];
+            if (columns != rows) s += sums[(r + rows) * kSumStride + j] + sums[(r + 2 * rows) * kSumStride + j];
             s *= kQ4Back<BF16>;
-            if (!isfinite(s)) s = plain_dot(p, r0 + r, first_row + lane);
-            store_real(p.Y, (r0 + r) * p.ldy + first_row + lane, p.type_y, s);
+            if (!isfinite(s)) s = plain_dot(p, r0 + r, first_row + j);
+            store_real(p.Y, (r0 + r) * p.ldy + first_row + j, p.type_y, s);
           }
         if (parts == 1) __syncwarp();
       }
@@ -573,16 +576,16 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
     if (p.slices > 1) {
       cluster_barrier();
       // this block's share of the outputs of its own units, from the sums of all blocks
-      const int outputs = workers_here * rows * kQ4Rows;
+      const int outputs = workers_here * rows * kRows;
       for (int at = slice * kThreads + tid; at < outputs; at += p.slices * kThreads) {
-        const int j = at % kQ4Rows, r = at / kQ4Rows % rows, l = at / kQ4Rows / rows;
-        const long long row = (static_cast<long long>(worker - local + l) + static_cast<long long>(round) * workers) * kQ4Rows + j;
+        const int j = at % kRows, r = at / kRows % rows, l = at / kRows / rows;
+        const long long row = (static_cast<long long>(worker - local + l) + static_cast<long long>(round) * workers) * kRows + j;
         if (row >= p.n) continue;
-        const float* from = all_sums + l * buffers * kQ4Buffer<NT> + r * kQ4SumStride + j;
+        const float* from = all_sums + l * buffers * kBuffer + r * kSumStride + j;
         float s = 0.0f;
         for (int v = 0; v < p.slices; ++v) {
           float rest = 0.0f;
-          if (columns != rows) rest = load_cluster(from + rows * kQ4SumStride, v) + load_cluster(from + 2 * rows * kQ4SumStride, v);
+          if (columns != rows) rest = load_cluster(from + rows * kSumStride, v) + load_cluster(from + 2 * rows * kSumStride, v);
           s += load_cluster(from, v) + rest;
         }
         s *= kQ4Back<BF16>;
