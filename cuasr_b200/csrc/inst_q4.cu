@@ -43,11 +43,12 @@ Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, const int
         if (plan.panel_steps <= 0) continue;
         const int blocks = std::max(1, std::min((units + workers - 1) / workers, clusters[i]));
         const double rounds = static_cast<double>(((units + workers - 1) / workers + blocks - 1) / blocks) * passes;
-        // In microseconds, from measurements between 1024 x 1024 and 128000 x 4096: a warp's step with all warps at it 1.7 (16 of
-        // them; 1.4 with eight, 2 for 32 columns), a worker's sums 1.3, a cluster's 2 more; X laid out by a block 0.5 for a step of
-        // all its columns' warps.  (One row, 14336 x 4096: 12.4 with four parts, 13.9 with eight, 17 with two.  Eight rows, 128000
-        // x 4096: 63 with one part, 65 with four.  Sixteen: 97 with eight warps, whose shared memory holds X, 198 with
-        // sixteen.  Thirty-two rows, 8192 x 8192: 38 with four slices of one part, 48 with two of two, 84 with two parts.)
+        // In microseconds, from measurements between 1024 x 1024 and 128000 x 4096: a warp's step with all warps at it 1.7 (1.4 where
+        // they are eight, 2 for 32 columns), a worker's sums 1.3, a cluster's 2 more; X laid out by a block 0.5 for a step of all its
+        // columns' warps.  Every plan was timed for 24 shapes; the chosen one was the best or within 5 % of it for 20 of them.  (One
+        // row, 14336 x 4096: 12.2 with four parts of 16 warps, 12.4 with two of two slices.  Eight rows, 128000 x 4096: 61.5 with one
+        // part, 63.9 with two, 70 with eight.  Sixteen: 90 with two parts, 96 with one.  Thirty-two rows, 8192 x 8192: 35 with four
+        // slices of one part, 41 with two of two, 60 with four parts.)
         const double step = shape.column_tiles == 4 ? 2.0 : warps == 16 ? 1.7 : 1.4;
         const double restaged = plan.panel_steps < slice_steps ? rounds : passes;
         const double cost = rounds * ((slice_steps + parts - 1) / parts * step + (parts > 1 ? 1.3 : 1.0) + (s > 1 ? 2.0 : 0.0)) +

@@ -21,14 +21,23 @@
 // AND-OR yields the pairs (k, k + 4), (k + 1, k + 5), ...  So a lane takes whole words of a weight row as they lie, and X is
 // laid out in shared memory, once per block, in the order that matches.
 //
-// A worker of 1, 2, 4 or 8 warps has 32 weight rows at a time; its warps take the steps of 256 k in turn and put their sums
-// together in shared memory.  Workers do not wait for one another (but for clusters, below).  Every warp has a pipeline of
-// its own: its steps (4 KB) come into its stages by TMA, issued by its first lane as soon as a stage has been read, across
-// the ends of a worker's rows too, so that the memory does not wait for sums.  Weight rows that TMA cannot describe (not on
-// 16-byte boundaries) are copied by the lanes in aligned words (cp.async) and shifted into place when they are read.
+// A worker of 1, 2, 4 or 8 warps has 32 weight rows at a time, or 16 where X has more than eight columns (whose sums take the
+// registers: 32 rows by 32 columns leave room for eight warps of an SM, 16 rows for sixteen; 4096 x 4096 by 32 rows of X 14.2 us
+// instead of 16.1).  Its warps take the steps of 256 k in turn and put their sums together in shared memory.  Workers do not wait for
+// one another (but for clusters, below).  Every warp has a pipeline of its own: its steps (4 KB, or 2) come into its two stages by
+// TMA, issued by its first lane as soon as a stage has been read, across the ends of a worker's rows too, so that the memory does not
+// wait for sums.  Weight rows that TMA cannot describe (not on 16-byte boundaries) are copied by the lanes in aligned words (cp.async)
+// and shifted into place when they are read.
 //
-// Where there are few weight rows for the SMs, or X is too large for a block's shared memory, the blocks of a cluster share
-// k, and their sums meet through distributed shared memory.
+// Where there are few weight rows for the SMs, or X is too large for a block's shared memory, the blocks of a cluster share k, and
+// their sums meet through distributed shared memory.
+//
+// What bounds it: for large n the instructions of a step (eight rows, 128000 x 4096: 60.7 us, 4.5 TB/s; the same pipeline without the
+// products 45 us); with more columns of X the chain of a warp's instructions, neither their number, nor the products (a third of the
+// rate of mma.sync), nor the reads of X, each of which was taken out in a trial without a gain; for small n what precedes the products
+// (the launch, X laid out: 2 to 8 us).  Tried and slower: three stages, one box of 128 bytes instead of two of 64, clusters of eight
+// (15 run at a time: 32 rows, 8192 x 8192 57 us instead of 35), more loads of X in flight (the registers), all products of one pair
+// before those of the other.
 #pragma once
 
 #include "../../include/cuasr_b200_types.h"
@@ -387,7 +396,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
     if constexpr (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (!TMA || lane == 0)
-    for (int s = 0; s < (TMA ? kQ4Stages : kQ4Stages - 1); ++s) copy_ahead();
+    for (int s = 0; s < kQ4Stages; ++s) copy_ahead();
 
   // Scales and zero points of a step, loaded one step ahead, for both its halves.  Where half a step has one group, lane
   // (g, t) has those of row t * 8 + g (of two tiles; of one, t and t + 2 have the same); else those of its t-th group for rows g, 8 + g, ...
@@ -463,7 +472,6 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
         if constexpr (TMA) {
           mbar_wait_or_abandon(&full[warp][stage], parity, p.status, kDeviceTimeoutFull, &abandoned);
         } else {
-          copy_ahead();                // into the stage that was read last
           asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 1) : "memory");
           __syncwarp();
         }
@@ -526,9 +534,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
           }
         }
         __syncwarp();                  // the stage has been read
-        if constexpr (TMA) {
-          if (lane == 0) copy_ahead();
-        }
+        if (!TMA || lane == 0) copy_ahead();
         if (++stage == kQ4Stages) { stage = 0; parity ^= 1; }
       }
     }
