@@ -403,9 +403,14 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
 }
 
 // One block per search: log-sums of its prefixes, then the best of all parts' candidates.  A part's candidates are a sorted list
-// of `keep`; a warp merges up to 32 of them by taking the largest head `keep` times, and the first warp merges what the
-// warps found.  What bounds this is the chain of steps, about 0.1 us for each that is kept, so a step is made short: the
-// candidates' values are worked out beforehand, as whole numbers, and a step is one maximum over a warp.
+// of `keep`, and the values of all of them are worked out as whole numbers, beforehand.
+//
+// Up to 32 lists are merged by a warp, which takes the largest of their heads `keep` times: a chain of 0.1 us for each (one maximum
+// over the warp).  With more lists that took two such chains, and the following is faster (5 searches of 91 lists, keep = 14: 11.9
+// us for the step instead of 14.6; with 32 lists, keep = 8, 24.2 instead of 22.2): the lists' first entries, 64 or more, are
+// compared with one another; the `keep`-th of these is a bound that `keep` candidates reach, and those of all lists that reach it
+// are sorted by comparing all with all.  Where more than 256 reach it (most of them equal), and where the lists do not fit into
+// shared memory, the warps share the lists.
 //
 // Whole numbers that order as the values do; 0 for -infinity and NaN.
 __device__ __forceinline__ unsigned long long beam_order(double value) {
@@ -445,18 +450,18 @@ __device__ __forceinline__ int warp_first(const BeamEntry& e) {
   return __ffs(who) - 1;
 }
 
-// An entry while lists are merged: list * keep + place of where it came from stands for its key.
+// A candidate in shared memory, without its key.
 struct __align__(16) BeamMerged {
   unsigned long long order;
-  int beam, from;
+  int beam, pad;
 };
 
-// Takes `keep` times the lane's head that comes first; entry(at) is the lane's at-th (order 0 behind its last), and of equal
-// ones of one beam key(from) decides.  taken[n] gets the entries' `from`, -1 behind the last.
-template <typename Entry, typename Key>
-__device__ __forceinline__ void merge_heads(int* taken, int keep, Entry entry, Key key) {
+// Takes `keep` times the lane's head that comes first; entry(at) is the lane's at-th (order 0 behind its last), and of equal ones of
+// one beam key(at) decides.  taken[n] gets place(at), -1 behind the last.
+template <typename Entry, typename Key, typename Place>
+__device__ __forceinline__ void merge_heads(int* taken, int keep, Entry entry, Key key, Place place) {
   const int lane = threadIdx.x % 32;
-  int at = 1, n = 0;
+  int at = 0, n = 0;
   BeamMerged e = entry(0), next = entry(1);
   for (; n < keep; ++n) {
     const unsigned int hi = static_cast<unsigned int>(e.order >> 32), top = __reduce_max_sync(0xFFFFFFFFu, hi);
@@ -469,31 +474,44 @@ __device__ __forceinline__ void merge_heads(int* taken, int keep, Entry entry, K
       if ((who & (who - 1)) != 0) {
         const int first = __reduce_min_sync(0xFFFFFFFFu, in ? e.beam : 0x7FFFFFFF);
         in = in && e.beam == first;
-        const unsigned long long mine = in ? key(e.from) : 0ull, largest = warp_max(mine);
+        const unsigned long long mine = in ? key(at) : 0ull, largest = warp_max(mine);
         who = __ballot_sync(0xFFFFFFFFu, in && mine == largest);
       }
     }
     if (lane == __ffs(who) - 1) {
-      taken[n] = e.from;
+      taken[n] = place(at);
       e = next;
-      next = entry(++at);
+      next = entry(++at + 1);
     }
   }
   for (n += lane; n < keep; n += 32) taken[n] = -1;
+}
+
+__host__ __device__ constexpr int beam_merge_scratch(int keep) {
+  const int picked = kMergeThreads * static_cast<int>(sizeof(BeamMerged) + sizeof(unsigned long long));
+  const int found = (1 + kMergeThreads / 32) * keep * static_cast<int>(sizeof(BeamEntry));
+  return picked > found ? picked : found;
 }
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamParams p) {
   extern __shared__ __align__(16) unsigned char beam_smem[];
   constexpr int kWarps = kMergeThreads / 32;
   const int lists = p.beams * p.parts, entries = lists * p.keep;                  // at most 1024 + 1036 lists
-  const bool merged = entries <= kBeamMergeMost && lists <= 32 * kWarps;
+  const bool merged = entries <= kBeamMergeMost && lists <= kMergeThreads;
+  __shared__ unsigned int bound;
+  __shared__ int n_picked;
+  // A block's shared memory is to fit beside the part kernel's blocks, whose places it otherwise takes while it waits for them (64
+  // searches of 16 prefixes over 64000 logits: 68 us instead of 64), so what is not needed at a time lies in one place.
   BeamMerged* here = reinterpret_cast<BeamMerged*>(beam_smem);                    // [lists][keep], if they fit
-  double* base = reinterpret_cast<double*>(here + (merged ? entries : 0));        // [beams]: score, less the log-sum
-  BeamEntry* found = reinterpret_cast<BeamEntry*>(base + p.beams);                // [1 + warps][keep]: the result, what each warp found;
-  int* taken = reinterpret_cast<int*>(found);                                     // where lists fit, as places in `here`
-  unsigned char* place = reinterpret_cast<unsigned char*>(merged ? static_cast<void*>(taken + (1 + kWarps) * p.keep)
-                                                                 : static_cast<void*>(found + (1 + kWarps) * p.keep));
-  unsigned char* done = place + (merged ? 0 : lists);                             // [beams], behind [lists]: how far each has been taken
+  unsigned char* scratch = beam_smem + (merged ? entries * sizeof(BeamMerged) : 0);
+  uint4* tops = reinterpret_cast<uint4*>(scratch);                                // first the entries that give the bound,
+  BeamMerged* picked = reinterpret_cast<BeamMerged*>(scratch);                    // then those that reach it and their keys,
+  unsigned long long* picked_key = reinterpret_cast<unsigned long long*>(picked + kMergeThreads);
+  int* taken = reinterpret_cast<int*>(scratch);                                   // or [keep], as places in `here`,
+  BeamEntry* found = reinterpret_cast<BeamEntry*>(scratch);                       // or [1 + warps][keep]: the result, what each warp found
+  double* base = reinterpret_cast<double*>(scratch + beam_merge_scratch(p.keep)); // [beams]: score, less the log-sum
+  unsigned char* place = reinterpret_cast<unsigned char*>(base + p.beams);        // [lists]: how far each has been taken
+  unsigned char* done = place + lists;                                            // [beams]
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, batch = blockIdx.x;
   grid_dependency_wait();
   grid_dependency_launch();
@@ -503,28 +521,23 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
   unsigned long long keys[kMine];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) keys[i] = i * kMergeThreads + tid < entries ? far[i * kMergeThreads + tid] : 0;
-  for (int b = warp; b < p.beams; b += kWarps) {
-    const long long part0 = (static_cast<long long>(batch) * p.beams + b) * p.parts;
-    const bool ended = p.finished != nullptr && p.finished[batch * p.ld_finished + b] != 0;
-    double value = p.scores[batch * p.ld_scores + b];
-    if (p.normalise) {             // an ended prefix has no sums: what is read for it is not used
-      float m = lane < p.parts ? p.part_max[part0 + lane] : -INFINITY, all = m;
-      double s = lane < p.parts ? p.part_sum[part0 + lane] : 0.0;
-      for (int i = lane + 32; i < p.parts; i += 32) all = fmaxf(all, p.part_max[part0 + i]);
-#pragma unroll
-      for (int o = 16; o > 0; o /= 2) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
-      auto scaled = [&](double sum, float max) {
-        return max == all || max == -INFINITY ? sum : sum * exp(static_cast<double>(max) - static_cast<double>(all));
-      };
-      s = scaled(s, m);
-      for (int i = lane + 32; i < p.parts; i += 32) s += scaled(p.part_sum[part0 + i], p.part_max[part0 + i]);
-      if (p.parts > 1) {
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-      }
-      if (!ended) value -= (all == -INFINITY ? 0.0 : static_cast<double>(all)) + log(s);
+  int group = 1;                   // lanes of a prefix, one for each of its parts (at most 32)
+  while (group < p.parts) group *= 2;
+  for (int b0 = warp * (32 / group); b0 < p.beams; b0 += kWarps * (32 / group)) {
+    const int b = b0 + lane / group, i = lane % group;
+    const bool mine = b < p.beams, some = mine && i < p.parts && p.normalise;    // an ended prefix has no sums: what is read for it is not used
+    const long long item = (static_cast<long long>(batch) * p.beams + b) * p.parts + i;
+    const float m = some ? p.part_max[item] : -INFINITY;
+    double s = some ? p.part_sum[item] : 0.0, value = mine ? p.scores[batch * p.ld_scores + b] : 0.0;
+    const bool ended = mine && p.finished != nullptr && p.finished[batch * p.ld_finished + b] != 0;
+    if (p.normalise) {
+      float all = m;
+      for (int o = group / 2; o > 0; o /= 2) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+      if (m != all && m != -INFINITY) s *= exp(static_cast<double>(m) - static_cast<double>(all));
+      for (int o = group / 2; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      if (!ended && i == 0) value -= (all == -INFINITY ? 0.0 : static_cast<double>(all)) + log(s);
     }
-    if (lane == 0) { base[b] = value; done[b] = ended; }
+    if (mine && i == 0) { base[b] = value; done[b] = ended; }
   }
   __syncthreads();
 
@@ -547,43 +560,86 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
   if (merged) {
     auto enter = [&](int e, unsigned long long key) {
       const int l = e / p.keep, b = l / p.parts;
-      here[e] = {work_out(l, b, e - l * p.keep, key).order, b, e};
+      here[e] = {work_out(l, b, e - l * p.keep, key).order, b, 0};
     };
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
       if (i * kMergeThreads + tid < entries) enter(i * kMergeThreads + tid, keys[i]);
     for (int e = kMine * kMergeThreads + tid; e < entries; e += kMergeThreads) enter(e, far[e]);
+    if (tid == 0) {
+      n_picked = 0;
+      bound = 0xFFFFFFFFu;
+    }
     __syncthreads();
-    auto key = [&](int from) { return far[from]; };        // (an ended prefix has one entry: its key is not asked for)
-    const BeamMerged none = {0, 0, -1};
-    const int warps = (lists + 31) / 32;
-    int* const mine = taken + (warps > 1 ? (1 + warp) * p.keep : 0);
-    if (warp < warps) {
-      const int first = lists * warp / warps, last = lists * (warp + 1) / warps, l = first + lane;
-      merge_heads(mine, p.keep, [&](int at) { return l < last && at < p.keep ? here[l * p.keep + at] : none; }, key);
-    }
-    if (warps > 1) {
-      __syncthreads();
-      if (warp == 0) {
-        const int* theirs = taken + (1 + lane) * p.keep;
-        merge_heads(taken, p.keep, [&](int at) {
-          const int from = lane < warps && at < p.keep ? theirs[at] : -1;
-          return from >= 0 ? here[from] : none;
-        }, key);
-      }
-    }
-    __syncwarp();
-    if (warp == 0)
-      for (int n = lane; n < p.keep; n += 32) {
-        const int from = taken[n];
+    if (lists <= 32) {
+      if (warp > 0) return;
+      const int mine = lane * p.keep;
+      const BeamMerged none = {0, -1, 0};
+      merge_heads(taken, p.keep, [&](int at) { return lane < lists && at < p.keep ? here[mine + at] : none; }, [&](int at) { return far[mine + at]; },
+                  [&](int at) { return mine + at; });
+      __syncwarp();
+      for (int i = lane; i < p.keep; i += 32) {
+        const int from = taken[i];
         const BeamMerged e = from >= 0 ? here[from] : none;
-        put(n, e.order, e.beam, from < 0 ? -1 : done[e.beam] ? p.end_token : beam_key_token(far[from]));
+        put(i, e.order, e.beam, from < 0 ? -1 : done[e.beam] ? p.end_token : beam_key_token(far[from]));
       }
-    return;
+      return;
+    }
+    const int depth = min(p.keep, max(1, max(64, 2 * p.keep) / lists)), items = lists * depth;
+    const unsigned int top = tid < items ? static_cast<unsigned int>(here[tid / depth * p.keep + tid % depth].order >> 32) : 0;
+    reinterpret_cast<unsigned int*>(tops)[tid] = top;
+    __syncthreads();
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < (items + 3) / 4; ++j) {
+      const uint4 v = tops[j];
+      above += (v.x > top) + (v.y > top) + (v.z > top) + (v.w > top);
+    }
+    const unsigned int least = __reduce_min_sync(0xFFFFFFFFu, tid < items && above < p.keep ? top : 0xFFFFFFFFu);
+    if (lane == 0) atomicMin(&bound, least);
+    __syncthreads();
+    const unsigned int reached = max(bound, 1u);   // of a value above -infinity the upper half is not 0
+    auto pick = [&](int e, auto&& key) {           // one entry of each thread, or none
+      const bool in = e < entries && static_cast<unsigned int>(here[e].order >> 32) >= reached;
+      const unsigned int who = __ballot_sync(0xFFFFFFFFu, in);
+      if (who == 0) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&n_picked, __popc(who));
+      at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(who & ((1u << lane) - 1));
+      if (in && at < kMergeThreads) {
+        picked[at] = here[e];
+        picked_key[at] = key();
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (i * kMergeThreads < entries) pick(i * kMergeThreads + tid, [&] { return keys[i]; });
+    for (int e = kMine * kMergeThreads + tid; e - tid < entries; e += kMergeThreads) pick(e, [&] { return far[e]; });
+    __syncthreads();
+    const int n = n_picked;
+    if (n <= kMergeThreads) {
+      int share = 1;               // threads of a candidate, each of which compares it with some of the others
+      while (share < 32 && 2 * share * n <= kMergeThreads) share *= 2;
+      const int i = min(tid / share, n - 1);
+      if (n > 0) {
+        const BeamMerged mine = picked[i];
+        const unsigned long long key = picked_key[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = tid % share; j < n; j += share) {
+          const BeamMerged other = picked[j];
+          const bool first = (other.beam < mine.beam) | ((other.beam == mine.beam) & (picked_key[j] > key));
+          rank += (other.order > mine.order) | ((other.order == mine.order) & first);
+        }
+        for (int o = share / 2; o > 0; o /= 2) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, o);
+        if (tid < n * share && tid % share == 0 && rank < p.keep) put(rank, mine.order, mine.beam, done[mine.beam] ? p.end_token : beam_key_token(key));
+      }
+      for (int left = n + tid; left < p.keep; left += kMergeThreads) put(left, 0, -1, -1);
+      return;
+    }
   }
 
-  // More candidates than shared memory holds: the warps share the lists, a warp takes the largest head of its own `keep`
-  // times, and the first merges what they found.
+  // The warps share the lists, a warp takes the largest head of its own `keep` times, and the first merges what they found.
   auto entry_of = [&](int l, int b, int at) {
     return at < p.keep ? work_out(l, b, at, far[static_cast<long long>(l) * p.keep + at]) : BeamEntry{0, 0, b, 0};
   };

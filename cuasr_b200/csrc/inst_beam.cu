@@ -70,11 +70,10 @@ cudaError_t launch_beam(const cuasr_b200_beam_args_t& a, const DeviceInfo& dev, 
   ++*launches;
   const int lists = a.beams * p.parts, entries = lists * a.keep;
   const bool merged = entries <= kBeamMergeMost && lists <= kMergeThreads;
-  const size_t smem = (merged ? entries * sizeof(BeamMerged) + (1 + kMergeThreads / 32) * a.keep * sizeof(int)
-                              : (1 + kMergeThreads / 32) * a.keep * sizeof(BeamEntry) + lists) + a.beams * (sizeof(double) + 1);
-  if (smem > 48 * 1024) {
+  const size_t smem = (merged ? entries * sizeof(BeamMerged) : 0) + beam_merge_scratch(a.keep) + a.beams * (sizeof(double) + 1) + lists;
+  if (smem > 47 * 1024) {             // the kernel has a few bytes of its own
     static std::atomic<uint64_t> allowed{0};
-    err = allow_shared_memory(reinterpret_cast<const void*>(beam_merge_kernel), 226 * 1024, allowed);
+    err = allow_shared_memory(reinterpret_cast<const void*>(beam_merge_kernel), 200 * 1024, allowed);
     if (err != cudaSuccess) return err;
   }
   err = launch_overlapped(beam_merge_kernel, a.batch, kMergeThreads, static_cast<int>(smem), 1, stream, p);
