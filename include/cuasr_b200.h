@@ -182,12 +182,12 @@ CUASR_B200_API int cuasr_b200_device_status(void *stream);
 /* A label for the last cuasr_b200_srgemm* call on this thread that depends on its arguments alone: "tma...", "path_tma" where
  * the storage lines of the operands (or of their copies) are what TMA can describe, "generic", "generic_splitk", "path" where
  * they are not; "..._splitk", "..._balanced", "..._repacked": what was asked for or had room in the workspace.  Which
- * kernel the call launched is answered by cuasr_b200_last_route. */
+ * kernel the call launched is answered by cuasr_b200_last_route.  "q4", "beam", "reorder": the calls of cuasr_b200_decode.h. */
 CUASR_B200_API const char *cuasr_b200_last_kernel(void);
 
 /* What the last cuasr_b200_srgemm* call on this thread launched: the kernel ("product", "screened", "path", "pack"; "none"
- * before the first call), its tile, the CTAs that share a tile's K through a cluster or in pieces, whether the pieces meet
- * through tickets in the workspace, and how each operand of the row-major problem came in ("tma", "tma-rows", "gather",
+ * before the first call; "q4", "beam", "reorder" after the calls of cuasr_b200_decode.h), its tile, the CTAs that share a tile's
+ * K through a cluster or in pieces, whether the pieces meet through tickets in the workspace, and how each operand of the row-major problem came in ("tma", "tma-rows", "gather",
  * "copy+tma"; with a column-major C that problem's operands are B and A), e.g.
  * "product tile=128x128 cluster=1 pieces=3 tickets=1 a=tma b=copy+tma".  "screened pieces=2 or product ...": both were launched, and
  * the values of the operands decided on the device which of them did the product.  For people and tests: the words may change.  The text

@@ -27,18 +27,23 @@ extern "C" {
 /* Y[r, j] = sum over k of X[r, k] * w[j, k],  w[j, k] = scale[j, k / group] * (q[j, k] - zero[j, k / group]).
  *
  * q[j, k] is the low (k even) or high (k odd) half of the byte W[j * ldw + k / 2]; zero is the low half of
- * zeros[j * ld_zeros + k / group], or 8 where `zeros` is NULL.  The differences are exact; the products of a group are
- * summed in 32 bits before the group's scale is applied, groups are summed in 32 bits, and Y is rounded once. */
+ * zeros[j * ld_zeros + k / group], or 8 where `zeros` is NULL.  With x as it is (32-bit values too), the sums of
+ * x q and of x of a group are taken in 32 bits, the scale is applied to  sum x q - zero sum x,  groups are summed in 32 bits, and Y is
+ * rounded once.  Sums of x q below 2^-103 (of F32 and BF16 values) may count as zero.  Outputs that are not finite in 32 bits are
+ * computed again element by element, so that infinities, NaN and values of 2^18 and more among the F32 and BF16 values are right, but
+ * slow: the outputs of a row of X with such a value take a thread each.
+ * Y must not share bytes with an operand.  The same call gives the same bits every time on one kind of device. */
 typedef struct cuasr_b200_q4_args {
   int32_t dtype_x;      /* CUASR_F32, CUASR_F16 or CUASR_BF16 */
   int32_t dtype_y;      /* the same choice */
   int32_t dtype_scale;  /* the same choice */
   int32_t group;        /* values along k that share a scale: a multiple of 32; at least k for one scale per row */
-  int32_t m, n, k;      /* X is m x k, W n x k, Y m x n; any sizes above 0.  Made for m up to 32 or so: the time of more
-                           rows grows with their number */
+  int32_t m, n, k;      /* X is m x k, W n x k, Y m x n; above 0, n and k at most 2^31 - 2^17, m at most 2 million (655350 rows of
+                           32 bits).  Made for m up to 32 or so: every 32 rows of X (10 of 32 bits) read the weights anew */
   int32_t device;
   const void *X;      int64_t ldx;        /* row-major; leading dimensions in elements, at least the row */
-  const uint8_t *W;   int64_t ldw;        /* bytes per row, at least (k + 1) / 2 */
+  const uint8_t *W;   int64_t ldw;        /* bytes per row, at least (k + 1) / 2; fastest where W and ldw are multiples of 16.  Bytes
+                                             between the rows may be read */
   const void *scales; int64_t ld_scales;  /* n x ceil(k / group) */
   const uint8_t *zeros; int64_t ld_zeros; /* n x ceil(k / group), or NULL */
   void *Y;            int64_t ldy;
@@ -54,7 +59,7 @@ CUASR_B200_API int cuasr_b200_q4_product(const cuasr_b200_q4_args_t *args);
  *   score[b] + logit[b, v]                              (normalise == 0: the inputs are log-probabilities)
  *   score[b] - log(sum over u of exp(logit[b, u])) + logit[b, v]        (normalise != 0)
  *
- * in 64-bit arithmetic, except for the exponentials (32 bits, summed in 32 bits along a few hundred of them, then in 64).
+ * in 64-bit arithmetic, except for the exponentials (32 bits, summed in 32 bits along a thread's few hundred of them, then in 64).
  * A prefix whose finished byte is not 0 has one continuation: `end_token`, with the prefix's own score.  Values of
  * -infinity and NaN are no continuations (a NaN or +infinity among the logits of a prefix thus ends it where they are
  * normalised).
@@ -64,7 +69,8 @@ CUASR_B200_API int cuasr_b200_q4_product(const cuasr_b200_q4_args_t *args);
 typedef struct cuasr_b200_beam_args {
   int32_t dtype;                       /* of the logits: CUASR_F32, CUASR_F16 or CUASR_BF16 */
   int32_t normalise;
-  int32_t batch, beams, vocab, keep;   /* all above 0; beams at most 1024, keep at most CUASR_B200_BEAM_MAX_KEEP */
+  int32_t batch, beams, vocab, keep;   /* all above 0; beams at most 1024, keep at most CUASR_B200_BEAM_MAX_KEEP, batch * beams at
+                                          most 2^24 */
   int32_t end_token;
   int32_t device;
   const void *logits;                  /* element (s, b, v) at s * batch_stride + b * beam_stride + v */
@@ -74,7 +80,7 @@ typedef struct cuasr_b200_beam_args {
   float *out_scores;   int64_t ld_out_scores;        /* batch x keep; may be `scores` itself, with the same leading
                                                         dimension */
   int32_t *parents;    int64_t ld_parents;           /* batch x keep */
-  int32_t *tokens;     int64_t ld_tokens;            /* batch x keep */
+  int32_t *tokens;     int64_t ld_tokens;            /* batch x keep; outputs share no bytes with anything else of the call */
   void *workspace;     size_t workspace_bytes;       /* cuasr_b200_beam_step_workspace_size bytes, 16-byte aligned; any
                                                         content, overwritten */
   void *stream;                                      /* cudaStream_t */
@@ -104,11 +110,11 @@ typedef struct cuasr_b200_state {
  * follow cuasr_b200_beam_step's back-pointers.  Positions behind lengths[s] of a ragged state and rows whose parent is
  * negative (places left over) stay as they were.  A parent of `beams` or more is not followed, and device status 4 is
  * recorded (cuasr_b200_device_status); lengths outside [0, positions] count as the nearer end.
- * In place: dst == src with equal strides, keep <= beams, and keep <= CUASR_B200_REORDER_MAX_IN_PLACE.  Otherwise the
+ * In place: dst == src with equal strides, rows that lie apart, keep <= beams, and keep <= CUASR_B200_REORDER_MAX_IN_PLACE.  Otherwise the
  * address ranges of src and dst must not meet.  No state's dst may share bytes with another state of the call (only equal
  * addresses are looked for), and the elements of a dst must lie apart. */
 typedef struct cuasr_b200_reorder_args {
-  int32_t batch, beams, keep;          /* above 0 */
+  int32_t batch, beams, keep;          /* above 0; keep at most 1024 */
   int32_t n_states;                    /* 0 to CUASR_B200_REORDER_MAX_STATES; 0 does nothing */
   const int32_t *parents; int64_t ld_parents;   /* batch x keep */
   const int32_t *lengths;              /* batch, or NULL where no state is ragged */
