@@ -58,31 +58,27 @@ bool plan_state(const cuasr_b200_state_t& s, const cuasr_b200_reorder_args_t& a,
   return true;
 }
 
-cudaError_t launch_some(const ReorderParams& p, unsigned int grid, cudaStream_t stream) {
+template <int STATES>
+cudaError_t launch_some(const ReorderParams<STATES>& p, unsigned int grid, cudaStream_t stream) {
   const int smem = p.keep * static_cast<int>(sizeof(int));
-  auto kernel = p.keep <= 4 ? reorder_kernel<4> : p.keep <= 8 ? reorder_kernel<8> : p.keep <= 16 ? reorder_kernel<16> : reorder_kernel<32>;
+  auto kernel = p.keep <= 4    ? reorder_kernel<4, STATES>
+                : p.keep <= 8  ? reorder_kernel<8, STATES>
+                : p.keep <= 16 ? reorder_kernel<16, STATES>
+                               : reorder_kernel<32, STATES>;
   return launch_overlapped(kernel, static_cast<int>(grid), kReorderThreads, smem, 1, stream, p);
 }
 
-}  // namespace
-
-bool reorder_fits(const cuasr_b200_reorder_args_t& a) {
-  ReorderState r;
-  for (int i = 0; i < a.n_states; ++i)
-    if (!plan_state(a.states[i], a, &r)) return false;
-  return true;
-}
-
-cudaError_t launch_reorder(const cuasr_b200_reorder_args_t& a, const DeviceInfo& dev, int* launches) {
-  ReorderParams p = {};
+template <int STATES>
+cudaError_t launch_states(const cuasr_b200_reorder_args_t& a, const DeviceInfo& dev, int* launches) {
+  ReorderParams<STATES> p;         // states behind the last are not looked at
   p.parents = a.parents; p.ld_parents = a.ld_parents; p.lengths = a.lengths; p.status = dev.status;
-  p.beams = a.beams; p.keep = a.keep;
+  p.beams = a.beams; p.keep = a.keep; p.states = 0;
   unsigned long long grid = 0;
   for (int i = 0; i < a.n_states; ++i) {
     ReorderState r;
     if (!plan_state(a.states[i], a, &r)) return cudaErrorInvalidValue;     // reorder_fits() was asked before
     const unsigned long long blocks = static_cast<unsigned long long>(r.blocks_per_batch) * a.batch;
-    if (p.states == kReorderStates || grid + blocks > 0x7FFFFFFFull) {
+    if (p.states == STATES || grid + blocks > 0x7FFFFFFFull) {
       const cudaError_t err = launch_some(p, static_cast<unsigned int>(grid), static_cast<cudaStream_t>(a.stream));
       if (err != cudaSuccess) return err;
       ++*launches;
@@ -96,6 +92,19 @@ cudaError_t launch_reorder(const cuasr_b200_reorder_args_t& a, const DeviceInfo&
   const cudaError_t err = launch_some(p, static_cast<unsigned int>(grid), static_cast<cudaStream_t>(a.stream));
   if (err == cudaSuccess) ++*launches;
   return err;
+}
+
+}  // namespace
+
+bool reorder_fits(const cuasr_b200_reorder_args_t& a) {
+  ReorderState r;
+  for (int i = 0; i < a.n_states; ++i)
+    if (!plan_state(a.states[i], a, &r)) return false;
+  return true;
+}
+
+cudaError_t launch_reorder(const cuasr_b200_reorder_args_t& a, const DeviceInfo& dev, int* launches) {
+  return a.n_states <= kReorderFew ? launch_states<kReorderFew>(a, dev, launches) : launch_states<kReorderStates>(a, dev, launches);
 }
 
 }  // namespace cuasr_b200

@@ -5,7 +5,9 @@
 
 namespace cuasr_b200 {
 
-constexpr int kReorderStates = 64;      // states of one launch
+// States of one launch; the parameters for eight are an eighth as large, which is host time (a call that reorders eight states of
+// 0.5 MB is over on the device in 3 us).
+constexpr int kReorderFew = 8, kReorderStates = 64;
 constexpr int kReorderThreads = 128;
 
 // A state as the kernel walks it: per search, `vectors` vectors of (1 << log_width) bytes for every beam; vector c lies in
@@ -22,32 +24,33 @@ struct ReorderState {
   unsigned int first_block, blocks_per_batch;
   unsigned char log_width, in_place, ragged, wide;   // wide: vector numbers pass 32 bits
 };
+template <int STATES>
 struct ReorderParams {
   const int* parents; long long ld_parents;
   const int* lengths;
   unsigned int* status;
   int beams, keep, states;
-  ReorderState state[kReorderStates];
+  ReorderState state[STATES];
 };
 
 // A column is one vector of every kept row: the thread that has it reads all it needs of the column before it writes, so
 // a search is reordered in place without a copy, and rows that stay where they are are neither read nor written.
 template <typename V, int ROWS>
-__device__ __forceinline__ void move_column(const ReorderParams& p, const char* src, char* dst, long long src_beam, long long dst_beam,
+__device__ __forceinline__ void move_column(int keep, const char* src, char* dst, long long src_beam, long long dst_beam,
                                             const int* from) {
-  for (int j0 = 0; j0 < p.keep; j0 += ROWS) {        // more than one round only where src and dst are apart
+  for (int j0 = 0; j0 < keep; j0 += ROWS) {        // more than one round only where src and dst are apart
     V v[ROWS];
 #pragma unroll
     for (int j = 0; j < ROWS; ++j)
-      if (j0 + j < p.keep && from[j0 + j] >= 0) v[j] = *reinterpret_cast<const V*>(src + from[j0 + j] * src_beam);
+      if (j0 + j < keep && from[j0 + j] >= 0) v[j] = *reinterpret_cast<const V*>(src + from[j0 + j] * src_beam);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j)
-      if (j0 + j < p.keep && from[j0 + j] >= 0) *reinterpret_cast<V*>(dst + (j0 + j) * dst_beam) = v[j];
+      if (j0 + j < keep && from[j0 + j] >= 0) *reinterpret_cast<V*>(dst + (j0 + j) * dst_beam) = v[j];
   }
 }
 
-template <int ROWS>
-__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderParams p) {
+template <int ROWS, int STATES>
+__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderParams<STATES> p) {
   extern __shared__ int from[];
   grid_dependency_wait();
   grid_dependency_launch();
@@ -90,11 +93,11 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
   char* dst = s.dst + batch * s.dst_batch + static_cast<long long>(segment) * s.dst_segment +
               static_cast<long long>(position) * s.dst_position + static_cast<long long>(offset);
   switch (s.log_width) {
-    case 4: move_column<uint4, ROWS>(p, src, dst, s.src_beam, s.dst_beam, from); break;
-    case 3: move_column<uint2, ROWS>(p, src, dst, s.src_beam, s.dst_beam, from); break;
-    case 2: move_column<unsigned int, ROWS>(p, src, dst, s.src_beam, s.dst_beam, from); break;
-    case 1: move_column<unsigned short, ROWS>(p, src, dst, s.src_beam, s.dst_beam, from); break;
-    default: move_column<unsigned char, ROWS>(p, src, dst, s.src_beam, s.dst_beam, from); break;
+    case 4: move_column<uint4, ROWS>(p.keep, src, dst, s.src_beam, s.dst_beam, from); break;
+    case 3: move_column<uint2, ROWS>(p.keep, src, dst, s.src_beam, s.dst_beam, from); break;
+    case 2: move_column<unsigned int, ROWS>(p.keep, src, dst, s.src_beam, s.dst_beam, from); break;
+    case 1: move_column<unsigned short, ROWS>(p.keep, src, dst, s.src_beam, s.dst_beam, from); break;
+    default: move_column<unsigned char, ROWS>(p.keep, src, dst, s.src_beam, s.dst_beam, from); break;
   }
 }
 
