@@ -40,6 +40,15 @@ def _device(buffers) -> Optional[int]:
     return found
 
 
+_NAMES = {DType.F32: ("float32",), DType.F16: ("float16",), DType.BF16: ("bfloat16",)}
+_BYTES, _FLAGS, _INDEX = ("uint8",), ("uint8", "bool"), ("int32",)
+
+
+def _typed(*buffers) -> bool:
+    """Whether every tensor has one of the element types named beside it; addresses have none."""
+    return all(str(x.dtype).rsplit(".", 1)[-1] in names for x, names in buffers if hasattr(x, "dtype"))
+
+
 @dataclasses.dataclass
 class Q4Arguments:
     """Y = X W^T: ref_X and ref_Y are row-major m x k and m x n, ref_W holds n rows of bytes (two weights each, the even k
@@ -147,16 +156,21 @@ class _DecodeOperator:
     def _required_workspace(self, packed) -> int:
         return 0
 
+    def _types_match(self, args) -> bool:
+        raise NotImplementedError
+
     def can_implement(self, args) -> Status:
-        packed = self._pack(args, None, None)
-        return Status.kErrorInvalidProblem if packed is None else _STATUS[self._can(ctypes.byref(packed))]
+        return self._check(args, self._pack(args, None, None))
+
+    def _check(self, args, packed) -> Status:
+        if packed is None:
+            return Status.kErrorInvalidProblem
+        return _STATUS[self._can(ctypes.byref(packed))] if self._types_match(args) else Status.kErrorInvalidDataType
 
     def initialize(self, args, workspace=None, stream=None) -> Status:
         """Checks the call and keeps it for run().  The operator keeps the buffers named in `args` alive."""
         packed = self._pack(args, workspace, stream)
-        if packed is None:
-            return Status.kErrorInvalidProblem
-        status = _STATUS[self._can(ctypes.byref(packed))]
+        status = self._check(args, packed)
         if status is Status.kSuccess and self._required_workspace(packed) > 0 and not packed.workspace:
             status = Status.kErrorWorkspaceNull
         if status is Status.kSuccess:
@@ -191,6 +205,10 @@ class Q4Product(_DecodeOperator):
         self.dtype_scale = self.dtype_x if dtype_scale is None else _real(dtype_scale)
         self.group = int(group)
 
+    def _types_match(self, args: Q4Arguments) -> bool:
+        return _typed((args.ref_X[0], _NAMES[self.dtype_x]), (args.ref_W[0], _BYTES), (args.ref_scales[0], _NAMES[self.dtype_scale]),
+                      (args.ref_zeros[0], _BYTES), (args.ref_Y[0], _NAMES[self.dtype_y]))
+
     def _pack(self, args: Q4Arguments, workspace, stream):
         m, n, k = args.problem_size
         refs = (args.ref_X, args.ref_W, args.ref_scales, args.ref_zeros, args.ref_Y)
@@ -208,6 +226,10 @@ class BeamStep(_DecodeOperator):
     def __init__(self, dtype: DType = DType.F32, normalise: bool = True):
         super().__init__()
         self.dtype, self.normalise = _real(dtype), bool(normalise)
+
+    def _types_match(self, args: BeamArguments) -> bool:
+        return _typed((args.ref_logits[0], _NAMES[self.dtype]), (args.ref_scores[0], _NAMES[DType.F32]), (args.ref_finished[0], _FLAGS),
+                      (args.ref_out_scores[0], _NAMES[DType.F32]), (args.ref_parents[0], _INDEX), (args.ref_tokens[0], _INDEX))
 
     def _pack(self, args: BeamArguments, workspace, stream):
         refs = (args.ref_scores, args.ref_finished, args.ref_out_scores, args.ref_parents, args.ref_tokens)
@@ -233,6 +255,9 @@ class BeamStep(_DecodeOperator):
 class ReorderStates(_DecodeOperator):
     """cuasr_b200_reorder_states."""
     _name = "cuasr_b200_reorder_states"
+
+    def _types_match(self, args: ReorderArguments) -> bool:
+        return _typed((args.ref_parents[0], _INDEX), (args.lengths, _INDEX))
 
     def _pack(self, args: ReorderArguments, workspace, stream):
         device = _device((args.ref_parents[0], args.lengths, *(x for s in args.states for x in (s.src, s.dst))))

@@ -204,6 +204,30 @@ def test_tensors_off_the_gpu_are_refused():
     assert ReorderStates().initialize(reorder_args([view(src=x)])) == Status.kErrorInvalidProblem
 
 
+class Typed:
+    """An address with an element type."""
+    def __init__(self, dtype):
+        self.dtype = dtype
+
+    def data_ptr(self):
+        return P
+
+
+def test_tensors_of_another_type_are_refused():
+    half, single, wide, flag = (Typed(t) for t in (torch.float16, torch.float32, torch.int64, torch.bool))
+    bad = Status.kErrorInvalidDataType
+    for change in ({"x": single}, {"w": half}, {"w": wide}, {"s": single}, {"y": single}, {"z": (half, 2)}):
+        op = Q4Product(DType.F16, group=32)
+        assert op.can_implement(q4_args(**change)) == bad and op.initialize(q4_args(**change)) == bad
+    for change in ({"logits": (half, 30, 10)}, {"scores": (half, 3)}, {"out": (half, 4)}, {"parents": (wide, 4)}, {"tokens": (single, 4)},
+                   {"finished": (wide, 3)}):
+        assert BeamStep().can_implement(beam_args(**change)) == bad and BeamStep().initialize(beam_args(**change), P) == bad
+    assert BeamStep().can_implement(beam_args(finished=(flag, 3), scores=(single, 3))) == Status.kSuccess
+    assert Q4Product(DType.F16, group=32).can_implement(q4_args(x=half, w=Typed(torch.uint8), y=half)) == Status.kSuccess
+    for change in ({"parents": (wide, 4)}, {"lengths": wide}):
+        assert ReorderStates().can_implement(reorder_args([view()], **change)) == bad
+
+
 def test_a_device_that_is_not_there_is_refused():
     packed = Q4Product(DType.F16, group=32)._pack(q4_args(), None, None)
     packed.device = 1000

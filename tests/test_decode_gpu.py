@@ -1,5 +1,9 @@
 """The decoding operators on the device against plain implementations in 64 bits."""
 import math
+import os
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -598,3 +602,70 @@ def test_two_searches_on_two_streams(cuda_device):
     for d, e in zip(alone, both):
         for a, b in zip(d.state(), e.state()):
             assert torch.equal(a, b)
+
+
+def test_the_first_calls_of_a_process_can_be_captured(cuda_device):
+    """In a process of its own: nothing is looked up on the device before the capture."""
+    code = """
+import sys
+sys.path.insert(0, "tests")
+import torch
+from test_decode_gpu import Decoder
+d, e = Decoder(25, vocab=20011), Decoder(25, vocab=20011)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    d.enqueue()
+for _ in range(2):
+    graph.replay()
+    e.enqueue()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(d.state(), e.state()))
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
+def test_calls_from_two_threads(cuda_device):
+    alone, both = [Decoder(seed) for seed in (26, 27)], [Decoder(seed) for seed in (26, 27)]
+    for d in alone:
+        for _ in range(20):
+            d.enqueue()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in both]
+    threads = [threading.Thread(target=lambda d=d, s=s: [d.enqueue(s) for _ in range(20)]) for d, s in zip(both, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    done()
+    for d, e in zip(alone, both):
+        for a, b in zip(d.state(), e.state()):
+            assert torch.equal(a, b)
+
+
+def test_replays_of_two_graphs_that_share_a_workspace(cuda_device):
+    """One after the other on one stream: the workspace is overwritten by every step."""
+    a, b, alone = Decoder(28), Decoder(29), [Decoder(28), Decoder(29)]
+    b.workspace = a.workspace
+    rows, vocab = (b.batch, b.beams), b.vocab
+    args = BeamArguments((*rows, vocab, b.beams), (b.q4.Y, b.beams * vocab, vocab), (b.scores, b.beams), (b.scores, b.beams),
+                         (b.parents, b.beams), (b.tokens, b.beams), (b.finished, b.beams))
+    assert b.step.initialize(args, a.workspace) == 0
+    graphs = []
+    for d in (a, b):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            d.enqueue()
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    for d in alone:
+        for _ in range(3):
+            d.enqueue()
+    done()
+    for d, e in zip((a, b), alone):
+        for x, y in zip(d.state(), e.state()):
+            assert torch.equal(x, y)
