@@ -248,16 +248,6 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
   int held = 0;                                          // candidates of this warp
   unsigned long long* segment = keys + warp * kBeamStride;
   __syncthreads();
-  // one logit of each lane (or none: -infinity) goes to the warp's candidates if it is above the bound
-  auto collect = [&](float value, int token, int room) {
-    const bool in = value > above;
-    const unsigned int who = __ballot_sync(0xFFFFFFFFu, in);
-    if (who != 0) {
-      const int at = held + __popc(who & ((1u << lane) - 1));
-      if (in && at < room) segment[at] = beam_key(value, token);
-      held += __popc(who);
-    }
-  };
   // the few logits outside of whole vectors, one to a lane of the first warp: those in front first, those behind last, so
   // that of equal logits the ones met later always have the higher token
   auto take_one = [&](int at, bool mine) {
@@ -267,7 +257,9 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
       sum = fmaf(sum, exp_of(m - ref), exp_of(value - ref));
     }
     m = m_new;
-    collect(value, at, kBeamStride);
+    const unsigned int who = __ballot_sync(0xFFFFFFFFu, value > above);
+    if (value > above) segment[held + __popc(who & ((1u << lane) - 1))] = beam_key(value, at);      // there is room for them
+    held += __popc(who);
   };
   if (part == 0 && head > 0 && warp == 0) take_one(lane, lane < head);
   int stage = 0, tile = 0;
@@ -311,14 +303,31 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
     }
     ++tile;
     if (__any_sync(0xFFFFFFFFu, top > above)) {
+      // which of a lane's logits are candidates, then where its first goes: one scan for all of them (one for each logit, by a
+      // ballot, took 2 us of the first tile)
+      unsigned int in = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (__any_sync(0xFFFFFFFFu, tops[u] > above)) {
           float v[V];
           unpack16(here[u * kBeamThreads], v, T());
 #pragma unroll
-          for (int e = 0; e < V; ++e) collect(v[e], head + (base + u * kBeamThreads + tid) * V + e, kBeamSegment);
+          for (int e = 0; e < V; ++e) in |= static_cast<unsigned int>(v[e] > above) << (u * V + e);
         }
+      const int count = __popc(in);
+      int at = count;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int before = __shfl_up_sync(0xFFFFFFFFu, at, o);
+        if (lane >= o) at += before;
+      }
+      const int found = __shfl_sync(0xFFFFFFFFu, at, 31);
+      for (at += held - count; in != 0; in &= in - 1, ++at) {
+        const int which = __ffs(in) - 1, u = which / V, e = which % V;
+        if (at < kBeamSegment)
+          segment[at] = beam_key(to_float(reinterpret_cast<const T*>(here + u * kBeamThreads)[e]), head + (base + u * kBeamThreads + tid) * V + e);
+      }
+      held += found;
     }
     if (__syncthreads_or(held > kBeamSegment)) {
       // more than the warp holds (many equal logits, or ever larger ones): what follows lies further along the row, and equal
