@@ -6,9 +6,8 @@
 // `keep` best; the searches' best are then chosen among those.  The floor is the logits' bytes at the memory's rate, which
 // leaves about eleven instructions of a lane for a 16-bit logit and twice as many for a 32-bit one; so exponentials are worked
 // out in pairs, and a logit is otherwise only part of a maximum, which is compared with a bound that nearly all threads stay
-// below.  The bound comes from the threads' own maxima and is taken
-// again after 1, 2, 4, ... tiles; a row of 16 tiles then has about seven candidates for each that is kept, which every warp
-// collects by itself and which are sorted once, at the row's end.
+// below.  The bound comes from the threads' own maxima and is taken again after 1, 2, 4, ... tiles; a row of 16 tiles then has
+// about seven candidates for each that is kept, which every warp collects by itself and which are sorted once, at the row's end.
 //
 // Measured: 64 searches of 16 prefixes over 64000 32-bit logits 58 us, 4.5 TB/s; 32 searches of four over 128000 16-bit logits, a
 // third of the prefixes ended, 19 us.  A block's later tiles pass at the memory's rate (2.3 thousand clocks with seven blocks to
