@@ -113,7 +113,8 @@ __device__ __forceinline__ float warp_jth(float x, int j) {
 }
 
 // A lower bound for the keep-th largest of the threads' values, where the first `warps` of the block have some: each has at
-// least keep / warps at or above its own, and the smallest of these bounds is taken.  All threads call it.
+// least keep / warps at or above its own, and the smallest of these bounds is taken.  All threads call it.  Between this call and
+// the next write to `scratch` lies a barrier: warps read it at the end.
 __device__ __forceinline__ float block_bound(float x, int keep, int warps, float* scratch) {
   const float mine = warp_jth(x, (keep + warps - 1) / warps);
   if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = mine;
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
   __shared__ unsigned long long keys[kBeamCapacity];
   __shared__ uint64_t full[kBeamStages];
   __shared__ int counter, counts[kBeamWarps];
-  __shared__ float maxima[kBeamWarps];
+  __shared__ float bounds[kBeamWarps], maxima[kBeamWarps];     // the bound's are still read when a warp that is ahead has its row's maximum
   __shared__ double sums[kBeamWarps];
   __shared__ unsigned int abandoned;
   constexpr int V = Vec16<T>::count, U = kBeamVectors, kTile = kBeamThreads * U;
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
     }
     m = m_new;
     if ((tile & (tile - 1)) == 0) {
-      const float bound = block_bound(m, p.keep, min((v_end - v_begin + 31) / 32, kBeamWarps), maxima);
+      const float bound = block_bound(m, p.keep, min((v_end - v_begin + 31) / 32, kBeamWarps), bounds);
       if (bound > floor) {
         floor = bound;
         above = float_below(bound);
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
   if (part == p.parts - 1 && tail > 0 && warp == 0) take_one(p.vocab - tail + lane, lane < tail);
 
   // what reaches the floor, one after the other
-  if (tile > 1) floor = fmaxf(floor, block_bound(m, p.keep, kBeamWarps, maxima));
+  if (tile > 1) floor = fmaxf(floor, block_bound(m, p.keep, kBeamWarps, bounds));
   static_assert(kBeamCapacity * sizeof(unsigned long long) <= kBeamStages * kBeamTileBytes, "the tiles' place is used");
   unsigned long long* sorted = reinterpret_cast<unsigned long long*>(beam_tiles);
   constexpr int kMine = (kBeamStride + 31) / 32;

@@ -389,6 +389,39 @@ def test_beam_step_many_prefixes(cuda_device, normalise, beams, keep):
     check_step(logits + torch.rand(2, beams, 50, generator=g, device="cuda") * normalise, scores, keep, normalise, finished)
 
 
+@pytest.mark.parametrize("normalise", [False, True])
+def test_beam_step_bound_at_the_end_of_a_row(cuda_device, normalise):
+    """Rows of three tiles whose eighth best is the second best of one warp, which holds the smallest bound and a maximum far above
+    it: every warp has to take that bound, however far the others are.  Each of 1024 rows, again and again."""
+    rows, lanes, tile = 1024, 128, 2048
+    x = torch.randn(rows, 3 * tile, generator=gen(40), device="cuda").clamp_(-2, 2) - 8
+    for poor in range(4):
+        for warp in range(4):
+            high = (6.5, 1.0) if warp == poor else (5.0 + warp / 8, 5.5 + warp / 8)
+            for lane, value in zip((32 * warp + poor, 32 * warp + 31 - poor), high):
+                x[poor::4, tile * (lane % 3) + lane * 4 + poor] = value
+    scores = torch.zeros(64, 16, device="cuda")
+    keep = 8
+    value, token = x.topk(keep, dim=1)
+    # the searches' best are among their prefixes' best, equal values of the lower prefix
+    at = value.view(64, -1).sort(dim=1, descending=True, stable=True)[1][:, :keep]
+    want = (at // keep).int(), token.view(64, -1).gather(1, at).int()
+    # searches of one prefix, too, whose outputs are all that the prefix has
+    for batch, beams in ((rows, 1),) if normalise else ((64, 16), (rows, 1)):
+        out = torch.empty(batch, keep, device="cuda")
+        parents, tokens = (torch.empty(batch, keep, device="cuda", dtype=torch.int32) for _ in range(2))
+        op = BeamStep(DType.F32, normalise)
+        args = BeamArguments((batch, beams, 3 * tile, keep), (x, beams * 3 * tile, 3 * tile), (scores, beams), (out, keep), (parents, keep), (tokens, keep))
+        workspace = torch.empty(op.get_workspace_size(args), device="cuda", dtype=torch.uint8)
+        assert op.initialize(args, workspace) == Status.kSuccess
+        wrong = torch.zeros((), device="cuda", dtype=torch.int64)
+        for _ in range(200):
+            assert op.run(torch.cuda.current_stream()) == Status.kSuccess
+            wrong += (tokens != (token if beams == 1 else want[1])).sum() + (parents != (0 if beams == 1 else want[0])).sum()
+        done()
+        assert wrong.item() == 0
+
+
 def test_beam_step_logits_beyond_32_bit_offsets(cuda_device):
     """Element offsets above 2^31: two searches whose rows lie 2^31 + 16 half-precision numbers apart."""
     far = 2 ** 31 + 16
