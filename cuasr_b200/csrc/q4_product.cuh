@@ -581,7 +581,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
             if (!isfinite(s)) s = plain_dot(p, r0 + r, first_row + j);
             store_real(p.Y, (r0 + r) * p.ldy + first_row + j, p.type_y, s);
           }
-        if (parts == 1) __syncwarp();
+        __syncwarp();                        // the lanes' loops differ in length; what follows are barriers of whole warps
       }
     }
     if (p.slices > 1) {
@@ -603,6 +603,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
         if (!isfinite(s)) s = plain_dot(p, r0 + r, row);
         store_real(p.Y, (r0 + r) * p.ldy + row, p.type_y, s);
       }
+      __syncwarp();                          // as above
       cluster_barrier();                     // no block writes its sums before all have read them
     }
   }

@@ -157,6 +157,21 @@ def test_q4_infinities_in_one_row(cuda_device, m, n, k, group, x):
     assert ((y[2:].double() - want[2:]).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("m,n,k,x", [(3, 40007, 700, DType.BF16), (7, 20011, 2304, DType.F16), (13, 12001, 4096, DType.BF16), (27, 20011, 4100, DType.F16),
+                                     (9, 15001, 1500, DType.F32), (32, 30005, 8192, DType.F16)])
+def test_q4_rounds_that_end_unevenly(cuda_device, m, n, k, x):
+    """Workers with several units of weight rows, the last of which is short, and numbers of rows of X that the warps cannot share
+    evenly: some lanes of a warp have an output more than others, and some of these are not finite."""
+    c = Q4Case(m, n, k, 128, x, DType.F32, pad=5, seed=n)
+    c.check()
+    first = c.Y.clone()
+    c.X[m // 2, k // 2] = math.nan
+    y = c.run()
+    done()
+    rest = torch.arange(m, device="cuda") != m // 2
+    assert torch.isnan(y[m // 2]).all() and torch.equal(y[rest], first[rest][:, :n])
+
+
 def test_q4_results_beyond_a_type(cuda_device):
     """Results that 16 bits do not hold become infinite, those of all zeros are zero."""
     c = Q4Case(3, 100, 256, 64, DType.BF16, DType.F16)
