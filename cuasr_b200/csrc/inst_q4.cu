@@ -7,23 +7,22 @@ namespace cuasr_b200 {
 namespace {
 
 struct Q4Plan {
-  int warps = 0, parts = 0, slices = 1, panel_steps = 0, grid = 0, sum_bytes = 0, xsum_bytes = 0, smem = 0;
+  int warps = 0, parts = 0, slices = 1, panel_steps = 0, grid = 0, sum_bytes = 0, smem = 0;
 };
-// What the shape of X and of the groups makes of a block.
+// What the shape of X makes of a block.
 struct Q4Shape {
-  int columns, column_tiles, rows, groups_per_step, stage_bytes;      // rows: weight rows of a worker
+  int columns, column_tiles, rows, stage_bytes;      // rows: weight rows of a worker
 };
 
 // Shared memory of a block: stages, sums, X of a panel and what is read behind it (X is read eight columns at a time).
 void fit(Q4Plan* plan, int slice_steps, const Q4Shape& s) {
   plan->sum_bytes = plan->warps / plan->parts * std::max(plan->parts - 1, 1) * s.column_tiles * 8 * (s.rows + kQ4SumPad) * 4;
-  const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64 + 16, all_stages = kQ4Stages * plan->warps * s.stage_bytes;
-  const int per_step = 512 * s.columns + 4 * s.groups_per_step * ((s.columns + 1) / 2 * 2), room = kQ4SmemPerBlock - fixed;
+  const int fixed = plan->sum_bytes + s.column_tiles * 8 * 64, all_stages = kQ4Stages * plan->warps * s.stage_bytes;
+  const int per_step = 512 * s.columns, room = kQ4SmemPerBlock - fixed;
   int panel = slice_steps;
   if (panel > (room - all_stages) / per_step) panel = (room - all_stages) / per_step / plan->parts * plan->parts;
   plan->panel_steps = panel;
-  plan->xsum_bytes = (4 * s.groups_per_step * ((s.columns + 1) / 2 * 2) * panel + 15) / 16 * 16;
-  plan->smem = fixed - 16 + plan->xsum_bytes + panel * 512 * s.columns + all_stages;
+  plan->smem = fixed + panel * per_step + all_stages;
 }
 
 // clusters[i]: clusters of 2^i blocks that the device runs at a time.
@@ -133,14 +132,14 @@ cudaError_t launch_q4(const cuasr_b200_q4_args_t& a, const DeviceInfo& dev, int*
   CUtensorMap map = {};
   const int tiles = nt == 1 ? 2 : 1;
   const bool tma = weight_map(&map, a, 16 * tiles);
-  const Q4Shape shape = {columns, nt, 16 * tiles, 8 / lw, (tma ? kQ4Stage<true, 1> : kQ4Stage<false, 1>) * tiles};
+  const Q4Shape shape = {columns, nt, 16 * tiles, (tma ? kQ4Stage<true, 1> : kQ4Stage<false, 1>) * tiles};
   p.units = (a.n - 1) / shape.rows + 1;
   int clusters[kQ4SliceChoices];
   cudaError_t err = count_clusters(clusters, dev.sms);
   if (err != cudaSuccess) return err;
   const Q4Plan plan = plan_q4(p.units, steps, passes, shape, clusters);
   if (plan.smem == 0) return cudaErrorInvalidValue;      // no launch fits: never for one block per SM and one slice
-  p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.sum_bytes = plan.sum_bytes; p.xsum_bytes = plan.xsum_bytes;
+  p.parts = plan.parts; p.slices = plan.slices; p.panel_steps = plan.panel_steps; p.sum_bytes = plan.sum_bytes;
   const Q4Launch l = {plan.grid, passes, plan.smem, static_cast<cudaStream_t>(a.stream)};
   err = nt == 4            ? launch_q4_columns<4, 1, 16>(lw, tma, map, p, l)
         : nt == 2          ? launch_q4_columns<2, 1, 16>(lw, tma, map, p, l)

@@ -3,19 +3,14 @@
 // The weights are read once, so the floor is their bytes at the memory's rate; at 6.5 TB/s that is 46 weights per SM and
 // clock, which leaves about ten instructions of a lane for eight weights.  Hence the tensor cores do the products
 // (mma.sync m16n8k16: sixteen weight rows by up to eight rows of X; an eighth of a tile is enough for one row, and the
-// instruction is not what bounds the kernel), and four bits become a factor by a single AND.  As the last bits of a 16-bit
-// number they are the subnormal q u, four places further up 16 q u, both exact (u = 2^-24 in binary16; 2^-133 in bfloat16,
-// where the numbers up to 255 u, the first normal ones among them, are still evenly spaced).
+// instruction is not what bounds the kernel), and two weights become factors by an AND and one multiply-add.  As the last bits of a
+// 16-bit number four bits are the subnormal q u, four places further up 16 q u, both exact (u = 2^-24 in binary16; 2^-133 in bfloat16,
+// where the numbers up to 255 u, the first normal ones among them, are still evenly spaced); times a power of two and less the zero
+// point they are (q - z) e, an exact number as well (e = 2^-9, 2^-6).  So the sums are those of the formula, in units of e: a
+// weight at its zero point adds nothing, and infinities and NaN of X go where the formula has them.  (Leaving zero points out of the products,
+// sum x q - z sum x, would save the multiply-add, but round against sum |x| q instead of sum |x (q - z)|.)
 //
-// A bfloat16 X is staged times 2^110, so that its products with such numbers lie well inside the range of 32 bits, and times
-// 2^106 where it meets a 16 q u; a 32-bit X as three such columns of 8 bits each, which sum up to it exactly.  A binary16 X is
-// staged as it is (a sixteenth of its smallest numbers could not be written) and the products with 16 q u are summed apart.
-// Infinities and NaN, and numbers from 2^18 on in the wide types, make every output of their row infinite or NaN: outputs
-// that are get computed once more as the formula has it.  At the other end the sums of x q end at 2^-103 (2^-126 in units of 2^-23).
-//
-// Zero points leave the products:  sum x (q - z) = sum x q - z sum x,  the sums of x by groups taken once per block, in 32
-// bits, where the accumulators start.  That costs the rounding of sum x q, about twice that of the result, and saves a
-// subtraction for two weights.
+// A 32-bit X is staged as three columns of 8 bits each, which sum up to it exactly (bits below 2^-133 are lost).
 //
 // The order of k inside a product is free as long as both operands have it.  A 32-bit word holds k, k + 1, ... k + 7; its
 // AND-OR yields the pairs (k, k + 4), (k + 1, k + 5), ...  So a lane takes whole words of a weight row as they lie, and X is
@@ -64,15 +59,11 @@ struct Q4Params {
   int rows;                                   // rows of X of a pass (blockIdx.y)
   int units, parts, slices;                   // 16 RT weight rows each; warps of a worker; blocks that share k
   int panel_steps;                            // steps whose X fits into shared memory; a multiple of parts if not all
-  int sum_bytes, xsum_bytes;
+  int sum_bytes;
   unsigned int* status;
   bool x_vectors;                             // X can be read 16 bytes at a time
 };
 
-__device__ __forceinline__ float load_real(const void* base, long long at, int type) {
-  return type == CUASR_F32 ? static_cast<const float*>(base)[at]
-         : type == CUASR_F16 ? to_float(static_cast<const __half*>(base)[at]) : to_float(static_cast<const __nv_bfloat16*>(base)[at]);
-}
 __device__ __forceinline__ void store_real(void* base, long long at, int type, float v) {
   if (type == CUASR_F32) static_cast<float*>(base)[at] = v;
   else if (type == CUASR_F16) static_cast<__half*>(base)[at] = __float2half_rn(v);
@@ -92,13 +83,33 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// The four pairs (k, k + 4) ... (k + 3, k + 7) of a word, the second and the fourth times 16.
-__device__ __forceinline__ void pairs_of(uint32_t w, uint32_t (&out)[4]) {
-  out[0] = w & 0x000F000Fu;
-  out[1] = w & 0x00F000F0u;
+// e: what q - z is multiplied by in a factor.
+template <bool BF16> constexpr float kQ4Unit = BF16 ? 0.015625f : 0.001953125f;       // 2^-6, 2^-9
+
+// a b + c of pairs; subnormal numbers are kept.
+template <bool BF16>
+__device__ __forceinline__ uint32_t fma_pair(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// The pair (v, v) of a whole number of units, at most 15 either way.
+template <bool BF16>
+__device__ __forceinline__ uint32_t unit_pair(int v) {
+  const float x = static_cast<float>(v) * kQ4Unit<BF16>;
+  if constexpr (BF16) return (__float_as_uint(x) >> 16) * 0x10001u;
+  else return __half_as_ushort(__float2half_rn(x)) * 0x10001u;
+}
+// The factors of the pairs (k, k + 4) ... (k + 3, k + 7) of a word; minus_z: unit_pair(-z).
+template <bool BF16>
+__device__ __forceinline__ void factors_of(uint32_t w, uint32_t minus_z, uint32_t (&out)[4]) {
+  constexpr uint32_t kUp = BF16 ? 0x7F007F00u : 0x78007800u, kUp16 = BF16 ? 0x7D007D00u : 0x68006800u;      // e / u, e / (16 u)
   const uint32_t upper = w >> 8;
-  out[2] = upper & 0x000F000Fu;
-  out[3] = upper & 0x00F000F0u;
+  out[0] = fma_pair<BF16>(w & 0x000F000Fu, kUp, minus_z);
+  out[1] = fma_pair<BF16>(w & 0x00F000F0u, kUp16, minus_z);
+  out[2] = fma_pair<BF16>(upper & 0x000F000Fu, kUp, minus_z);
+  out[3] = fma_pair<BF16>(upper & 0x00F000F0u, kUp16, minus_z);
 }
 
 // Memory word of half a step that word i of lane t of a quad is.  A group's products are summed apart, so the four lanes of an
@@ -213,23 +224,17 @@ __device__ __forceinline__ void load_x8(const Q4Params& p, long long row, int k,
   }
 }
 
-// What the products are multiplied by in the end.
-template <bool BF16> constexpr float kQ4Back = BF16 ? 8388608.0f : 16777216.0f;       // 2^23, 2^24
-
-// Lays out X for steps [begin, end): 16 bytes for each (half a step, word of a lane, column, lane of a quad), and -z times the
-// sums by groups (z = 8, or 1 where zero points are given).  Columns are the rows of X; a 32-bit row is three.
+// Lays out X for steps [begin, end): 16 bytes for each (half a step, word of a lane, column, lane of a quad).  Columns are the rows of
+// X; a 32-bit row is three.
 // Not inlined: it runs once a panel, and its registers are not to crowd out those of the products.
-template <bool BF16, typename E, int LW, int THREADS>
-__device__ __noinline__ void stage_x(const Q4Params& p, uint4* xs, float* xsums, int r0, int rows, int columns, int pitch, int begin, int end) {
+template <typename E, int LW, int THREADS>
+__device__ __noinline__ void stage_x(const Q4Params& p, uint4* xs, int r0, int rows, int columns, int begin, int end) {
   constexpr int kBatch = 4 / sizeof(E);                       // loads of as many items are in flight: more cost the kernel registers
-  constexpr int kLanes = LW * 4;                              // words of a group
   constexpr int kAtOnce = THREADS / 32;
-  const float z = (p.zeros == nullptr ? -8.0f : -1.0f) / kQ4Back<BF16>;
   const int lane = threadIdx.x % 32, steps = end - begin, in_half = lane % 16;
   const int i = LW == 4 ? in_half % 4 : LW == 2 ? in_half / 8 * 2 + in_half % 2 : in_half / 4;
   const int t = LW == 4 ? in_half / 4 : LW == 2 ? in_half / 2 % 4 : in_half % 4;
   uint4* const xs_lane = xs + (lane / 16 * 4 + i) * columns * 4 + t;
-  float* const sums_lane = xsums + (lane / 16 * (4 / LW) + in_half / kLanes) * pitch;
   // a warp takes a step of a row (32 words) at a time: row r, step s behind `begin`
   int r = threadIdx.x / 32 / steps, s = threadIdx.x / 32 % steps;
   auto next = [&](int& row, int& step) {
@@ -248,70 +253,32 @@ __device__ __noinline__ void stage_x(const Q4Params& p, uint4* xs, float* xsums,
     for (int q = 0; q < kBatch; ++q) {
       if (r >= rows) break;
       uint4* to = xs_lane + (s * 8 * columns + r) * 4;
-      float x[8];
-      if constexpr (sizeof(E) == 4) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(bits[q][e]);
-      } else {
-        const uint4 v = make_uint4(bits[q][0], bits[q][1], bits[q][2], bits[q][3]);
-        if constexpr (BF16) unpack16(v, x, __nv_bfloat16());
-        else unpack16(v, x, __half());
-      }
-      float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-      if (in_half % kLanes == 0) {
-        float* to_sum = sums_lane + s * (8 / LW) * pitch + r;
-        *to_sum = z * sum;
-        if constexpr (sizeof(E) == 4) to_sum[rows] = to_sum[2 * rows] = 0.0f;       // the whole sum goes with the first column
-      }
-      constexpr float up = 1.298074214633707e33f, up16 = up / 16;                   // 2^110
       if constexpr (sizeof(E) == 2) {
         const uint32_t(&v)[4] = bits[q];
-        uint4 pairs = make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410),
-                                 __byte_perm(v[1], v[3], 0x7632));
-        if constexpr (BF16) {
-          auto times = [](uint32_t a, float by) {
-            const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), __float2bfloat162_rn(by));
-            return *reinterpret_cast<const uint32_t*>(&h);
-          };
-          *to = make_uint4(times(pairs.x, up), times(pairs.y, up16), times(pairs.z, up), times(pairs.w, up16));
-        } else {
-          *to = make_uint4(pairs.x, pairs.z, pairs.y, pairs.w);       // the pairs that meet q first, then those that meet 16 q
-        }
+        *to = make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410),
+                         __byte_perm(v[1], v[3], 0x7632));
       } else {
+        uint32_t h[3][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= e % 2 == 0 ? up : up16;
-#pragma unroll
-        for (int part = 0; part < 3; ++part) {
-          uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            h[e] = __float_as_uint(x[e]) >> 16;                       // the upper half: a bfloat16, rounded towards zero
-            x[e] -= __uint_as_float(h[e] << 16);
-          }
-          to[part * rows * 4] = make_uint4(h[0] | h[4] << 16, h[1] | h[5] << 16, h[2] | h[6] << 16, h[3] | h[7] << 16);
+        for (int e = 0; e < 8; ++e) {
+          // the upper half is a bfloat16, rounded towards zero; what is left of an infinity or a NaN is nothing (a NaN stays one
+          // whichever of its bits are set)
+          const uint32_t all = bits[q][e];
+          const bool finite = (all & 0x7F800000u) != 0x7F800000u;
+          h[0][e] = finite || (all & 0x007FFFFFu) == 0 ? all >> 16 : 0x7FFFu;
+          float rest = finite ? __uint_as_float(all) - __uint_as_float(all & 0xFFFF0000u) : 0.0f;
+          h[1][e] = __float_as_uint(rest) >> 16;
+          rest -= __uint_as_float(h[1][e] << 16);
+          h[2][e] = __float_as_uint(rest) >> 16;
         }
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+          to[part * rows * 4] = make_uint4(h[part][0] | h[part][4] << 16, h[part][1] | h[part][5] << 16, h[part][2] | h[part][6] << 16,
+                                           h[part][3] | h[part][7] << 16);
       }
       next(r, s);
     }
   }
-}
-
-// Row r of X times weight row j as the formula has it.
-static __device__ __noinline__ float plain_dot(const Q4Params& p, int r, long long j) {
-  float sum = 0.0f;
-  for (int group = 0; group < p.groups; ++group) {
-    const int zero = p.zeros == nullptr ? 8 : p.zeros[j * p.ld_zeros + group] & 15;
-    const long long stop = min(static_cast<long long>(p.k), (group + 1LL) * p.group);
-    float part = 0.0f;
-    for (long long k = static_cast<long long>(group) * p.group; k < stop; ++k) {
-      const int q = p.W[j * p.ldw + k / 2] >> (k % 2 * 4) & 15;
-      part = fmaf(static_cast<float>(q - zero), load_real(p.X, r * p.ldx + k, p.type_x), part);
-    }
-    sum = fmaf(load_real(p.scales, j * p.ld_scales + group, p.type_scale), part, sum);
-  }
-  return sum;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -349,12 +316,10 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
   float* all_sums = reinterpret_cast<float*>(q4_smem + WARPS * kQ4Stages * kStage);
   const int buffers = max(parts - 1, 1);                   // of a worker
   float* sums = all_sums + local * buffers * kBuffer;
-  float* xsums = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(all_sums) + p.sum_bytes);
-  uint4* xs = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(xsums) + p.xsum_bytes);
+  uint4* xs = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(all_sums) + p.sum_bytes);
   const int slice = p.slices > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int r0 = blockIdx.y * p.rows, rows = min(p.rows, p.m - r0);
   const int columns = p.type_x == CUASR_F32 ? 3 * rows : rows;
-  const int pitch = (columns + 1) / 2 * 2;       // of xsums
   const int all_steps = (p.k + kQ4Step - 1) / kQ4Step;
   const int begin = static_cast<int>(static_cast<long long>(all_steps) * slice / p.slices);
   const int end = static_cast<int>(static_cast<long long>(all_steps) * (slice + 1) / p.slices);
@@ -453,24 +418,21 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
       const int panel_end = min(end, panel + p.panel_steps);
       if (!one_panel || round == 0) {
         if (!one_panel) __syncthreads();       // the panel before has been read
-        if constexpr (BF16) {
-          if (p.type_x == CUASR_F32) stage_x<true, uint32_t, LW, kThreads>(p, xs, xsums, r0, rows, columns, pitch, panel, panel_end);
-          else stage_x<true, unsigned short, LW, kThreads>(p, xs, xsums, r0, rows, columns, pitch, panel, panel_end);
-        } else {
-          stage_x<false, unsigned short, LW, kThreads>(p, xs, xsums, r0, rows, columns, pitch, panel, panel_end);
-        }
+        if (BF16 && p.type_x == CUASR_F32) stage_x<uint32_t, LW, kThreads>(p, xs, r0, rows, columns, panel, panel_end);
+        else stage_x<unsigned short, LW, kThreads>(p, xs, r0, rows, columns, panel, panel_end);
         __syncthreads();
       }
       if (!mine) continue;
       for (int step = panel + part_of; step < panel_end; step += parts) {
-        float scale[2][kMine], zero[2][kMine];
+        float scale[2][kMine];
+        uint32_t zero[2][kMine];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int j = 0; j < kMine; ++j) {
             scale[u][j] = p.type_scale == CUASR_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(next_scale[u][j])))
                                                     : __uint_as_float(next_scale[u][j] << scale_shift);
-            if constexpr (ZEROS) zero[u][j] = static_cast<float>(next_zero[u][j] & 15u);
+            if constexpr (ZEROS) zero[u][j] = unit_pair<BF16>(-static_cast<int>(next_zero[u][j] & 15u));
           }
         if (step + parts < end) load_scales(unit, step + parts);
         else load_scales(unit + workers, begin + part_of);
@@ -490,22 +452,18 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
             if constexpr (TMA) read_words<LW>(w[j], words, j, g, t);
             else read_words_shifted<LW>(w[j], words, j, g, t, shift[j]);
           }
-          const float* xsum = xsums + ((step - panel) * 2 + u) * (4 / LW) * pitch + t * 2;
-          constexpr int kSums = BF16 ? 1 : 2;            // products with q, and with 16 q
-          float part[kSums][RT][NT][4], f[2 * RT];
+          float part[RT][NT][4], f[2 * RT];
+          uint32_t minus_z[2 * RT];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float2 start[NT];
-            float z[2 * RT];
             if (i % LW == 0) {
 #pragma unroll
               for (int j = 0; j < 2 * RT; ++j) {
                 const int from = (lane & ~3) + (LW == 4 ? j : LW == 2 ? i / 2 * 2 : i), of = LW == 4 ? 0 : j;
                 f[j] = __shfl_sync(0xFFFFFFFFu, scale[u][of], from);
-                if constexpr (ZEROS) z[j] = __shfl_sync(0xFFFFFFFFu, zero[u][of], from);
+                if constexpr (ZEROS) minus_z[j] = __shfl_sync(0xFFFFFFFFu, zero[u][of], from);
+                else minus_z[j] = BF16 ? 0xBE00BE00u : 0xA400A400u;            // -8 e
               }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) start[nt] = *reinterpret_cast<const float2*>(xsum + i / LW * pitch + nt * 8);
             }
             uint4 b[NT];
 #pragma unroll
@@ -514,25 +472,18 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
               uint32_t lo[4], hi[4];
-              pairs_of(w[2 * rt][i], lo);
-              pairs_of(w[2 * rt + 1][i], hi);
-              const uint32_t a0[4] = {lo[0], hi[0], lo[BF16 ? 1 : 2], hi[BF16 ? 1 : 2]}, a1[4] = {lo[BF16 ? 2 : 1], hi[BF16 ? 2 : 1], lo[3], hi[3]};
+              factors_of<BF16>(w[2 * rt][i], minus_z[2 * rt], lo);
+              factors_of<BF16>(w[2 * rt + 1][i], minus_z[2 * rt + 1], hi);
+              const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                float(&d)[4] = part[0][rt][nt];
-                float(&d16)[4] = part[kSums - 1][rt][nt];
-                if (i % LW == 0) {
-                  const float2 s = start[nt];
-                  if constexpr (ZEROS) mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, z[2 * rt] * s.x, z[2 * rt] * s.y, z[2 * rt + 1] * s.x, z[2 * rt + 1] * s.y);
-                  else mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, s.x, s.y, s.x, s.y);
-                } else {
-                  mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, d[0], d[1], d[2], d[3]);
-                }
-                if (!BF16 && i % LW == 0) mma_16816<BF16>(d16, a1, b[nt].z, b[nt].w, 0.0f, 0.0f, 0.0f, 0.0f);
-                else mma_16816<BF16>(d16, a1, b[nt].z, b[nt].w, d16[0], d16[1], d16[2], d16[3]);
+                float(&d)[4] = part[rt][nt];
+                if (i % LW == 0) mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, 0.0f, 0.0f, 0.0f, 0.0f);
+                else mma_16816<BF16>(d, a0, b[nt].x, b[nt].y, d[0], d[1], d[2], d[3]);
+                mma_16816<BF16>(d, a1, b[nt].z, b[nt].w, d[0], d[1], d[2], d[3]);
                 if (i % LW == LW - 1) {
 #pragma unroll
-                  for (int c = 0; c < 4; ++c) acc[rt][nt][c] = fmaf(f[2 * rt + c / 2], BF16 ? d[c] : fmaf(d16[c], 0.0625f, d[c]), acc[rt][nt][c]);
+                  for (int c = 0; c < 4; ++c) acc[rt][nt][c] = fmaf(f[2 * rt + c / 2], d[c], acc[rt][nt][c]);
                 }
               }
             }
@@ -577,9 +528,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
           for (int r = part_of * (2 / RT) + lane / kRows; r < rows; r += parts * (2 / RT)) {
             float s = sums[r * kSumStride + j];
             if (columns != rows) s += sums[(r + rows) * kSumStride + j] + sums[(r + 2 * rows) * kSumStride + j];
-            s *= kQ4Back<BF16>;
-            if (!isfinite(s)) s = plain_dot(p, r0 + r, first_row + j);
-            store_real(p.Y, (r0 + r) * p.ldy + first_row + j, p.type_y, s);
+            store_real(p.Y, (r0 + r) * p.ldy + first_row + j, p.type_y, s * (1 / kQ4Unit<BF16>));
           }
         __syncwarp();                        // the lanes' loops differ in length; what follows are barriers of whole warps
       }
@@ -599,9 +548,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
           if (columns != rows) rest = load_cluster(from + rows * kSumStride, v) + load_cluster(from + 2 * rows * kSumStride, v);
           s += load_cluster(from, v) + rest;
         }
-        s *= kQ4Back<BF16>;
-        if (!isfinite(s)) s = plain_dot(p, r0 + r, row);
-        store_real(p.Y, (r0 + r) * p.ldy + row, p.type_y, s);
+        store_real(p.Y, (r0 + r) * p.ldy + row, p.type_y, s * (1 / kQ4Unit<BF16>));
       }
       __syncwarp();                          // as above
       cluster_barrier();                     // no block writes its sums before all have read them

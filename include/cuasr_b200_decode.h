@@ -27,12 +27,10 @@ extern "C" {
 /* Y[r, j] = sum over k of X[r, k] * w[j, k],  w[j, k] = scale[j, k / group] * (q[j, k] - zero[j, k / group]).
  *
  * q[j, k] is the low (k even) or high (k odd) half of the byte W[j * ldw + k / 2]; zero is the low half of
- * zeros[j * ld_zeros + k / group], or 8 where `zeros` is NULL.  With x as it is (32-bit values too), the sums of
- * x q and of x of a group are taken in 32 bits, the scale is applied to  sum x q - zero sum x,  groups are summed in 32 bits, and Y is
- * rounded once.  Sums of x q below 2^-103 (of F32 and BF16 values) may count as
- * zero, and results below 2^-102 lose bits.  Outputs that are not finite in 32 bits are
- * computed again element by element, so that infinities, NaN and values of 2^18 and more among the F32 and BF16 values are right, but
- * slow: the outputs of a row of X with such a value take a thread each.
+ * zeros[j * ld_zeros + k / group], or 8 where `zeros` is NULL.  With x as it is (32-bit values too) and q - zero as the whole
+ * number it is, the products are summed by groups in 32 bits, the scale is applied, groups are summed in 32 bits, and Y is rounded
+ * once.  Weights at their zero point add exactly nothing; infinities and NaN among the values reach the outputs that the formula
+ * gives them to.  Of F32 and BF16 values, bits below 2^-133 and products below 2^-120 may count as zero.
  * Y must not share bytes with an operand.  The same call gives the same bits every time on one kind of device. */
 typedef struct cuasr_b200_q4_args {
   int32_t dtype_x;      /* CUASR_F32, CUASR_F16 or CUASR_BF16 */

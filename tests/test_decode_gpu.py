@@ -157,6 +157,86 @@ def test_q4_infinities_in_one_row(cuda_device, m, n, k, group, x):
     assert ((y[2:].double() - want[2:]).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("x", REALS)
+@pytest.mark.parametrize("m,n,k,group", [(1, 70, 256, 64), (4, 300, 1000, 128), (3, 64, 4100, 8192), (11, 130, 640, 32), (20, 45, 2050, 128)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_q4_weights_at_their_zero_points(cuda_device, x, m, n, k, group, zeros):
+    """Weights that equal their zero point (padded or pruned ones) add nothing, not even a rounding, whatever the activations; few
+    others among them count as in Q4Case.check, whose bound goes by |x w|."""
+    for byte_offset in (0, 1):
+        c = Q4Case(m, n, k, group, x, DType.F32, zeros=zeros, pad=(-(k + 1) // 2) % 16, byte_offset=byte_offset, seed=k)
+        c.X += 3
+        c.X[0, ::5] = 1000.25
+        at = torch.arange(2 * c.W.shape[1], device="cuda").div(group, rounding_mode="floor").clamp_(max=-(-k // group) - 1)
+        zero = (c.zeros & 15)[:, at] if zeros else torch.full((n, at.numel()), 8, device="cuda", dtype=torch.uint8)
+        g = gen(n)
+
+        def weigh(q):
+            c.W.copy_(q[:, 0::2] | q[:, 1::2] << 4)
+        weigh(zero)
+        y = c.run()
+        done()
+        assert (c.weights() == 0).all() and torch.equal(y, torch.zeros_like(y))
+        # one in 64 lies beside the zero point
+        near = (torch.rand(zero.shape, generator=g, device="cuda") < 1 / 64).to(torch.uint8)
+        weigh(torch.where(zero == 15, zero - near, zero + near))
+        c.check()
+        # a large activation on weights of zero
+        c.X[:, k // 2] = 16384.0
+        c.W[:, k // 4] = zero[:, k // 4 * 2] | zero[:, k // 4 * 2 + 1] << 4
+        c.check()
+
+
+@pytest.mark.parametrize("x", REALS)
+@pytest.mark.parametrize("m", [1, 3, 10, 14])
+@pytest.mark.parametrize("k,group", [(128, 128), (500, 512), (4096, 4096)])
+def test_q4_one_weight_is_exact(cuda_device, x, m, k, group):
+    """A weight row with one number that is not zero, scales of 1: the output is that product, rounded once.  Every bit of a 32-bit
+    activation is in it."""
+    n = 61
+    c = Q4Case(m, n, k, group, x, DType.F32, zeros=True, seed=m)
+    c.scales.fill_(1)
+    c.X[:, ::3] *= 2.0 ** 10
+    c.X[:, 1::3] *= 2.0 ** -10
+    zero = (c.zeros & 15).expand(n, 2 * c.W.shape[1]).clone()
+    at = torch.randint(0, k, (n, 1), generator=gen(k), device="cuda")
+    zero.scatter_(1, at, torch.randint(0, 16, (n, 1), generator=gen(m), device="cuda", dtype=torch.uint8))
+    c.W.copy_(zero[:, 0::2] | zero[:, 1::2] << 4)
+    y = c.run()
+    done()
+    w = c.weights()
+    assert ((w != 0).sum(dim=1) <= 1).all() and (w != 0).any()
+    want = c.X.double()[:, at[:, 0]] * w.gather(1, at)[:, 0]      # 24 bits by four: exact in 64
+    assert torch.equal(y, want.float())
+
+
+def test_q4_non_finite_numbers_of_all_kinds(cuda_device):
+    """Infinities and NaN reach the outputs whose weight is not zero (all, of a NaN), whichever of a NaN's bits are set; neighbouring
+    rows and the largest finite numbers do not suffer."""
+    c = Q4Case(8, 200, 512, 64, DType.F32, zeros=True)
+    bits = c.X.view(torch.int32)
+    bits[0, 3], bits[1, 4], bits[2, 5], bits[3, 6] = 0x7F800001, 0x7FFFFFFF, -1, 0x7FC00000           # NaN
+    bits[4, 7], bits[5, 8] = 0x7F800000, 0x7F800000 - 2 ** 31                                         # infinities
+    c.X[6, 9], c.X[7, 10:12] = 3.4e38, 2.0 ** 20
+    y, w = c.run(), c.weights()
+    done()
+    assert torch.isnan(y[:4]).all()
+    assert (torch.isnan(y[4]) == (w[:, 7] == 0)).all() and (y[4] == INF).eq(w[:, 7] > 0).all() and (y[4] == -INF).eq(w[:, 7] < 0).all()
+    assert (torch.isnan(y[5]) == (w[:, 8] == 0)).all() and (y[5] == -INF).eq(w[:, 8] > 0).all() and (y[5] == INF).eq(w[:, 8] < 0).all()
+    want = c.X[6:].double() @ w.T
+    steps = 64 + 8 + 16                                                                               # as in Q4Case.check
+    assert ((y[6:].double() - want).abs() <= steps * 2.0 ** -23 * (c.X[6:].double().abs() @ w.abs().T) + 2.0 ** -24 * 1.001 * want.abs()).all()
+
+
+@pytest.mark.parametrize("x,size", [(DType.F16, 2.0 ** -22), (DType.BF16, 2.0 ** -100), (DType.F32, 2.0 ** -100)])
+def test_q4_small_activations(cuda_device, x, size):
+    """Subnormal half-precision activations, and ones for which 32 bits have room still, with scales that bring them back."""
+    c = Q4Case(3, 50, 300, 64, x, DType.F32, DType.F32, zeros=True)
+    c.X.copy_(torch.randn(3, 300, generator=gen(50), device="cuda") * size)
+    c.scales *= 2.0 ** 20
+    c.check()
+
+
 @pytest.mark.parametrize("m,n,k,x", [(3, 40007, 700, DType.BF16), (7, 20011, 2304, DType.F16), (13, 12001, 4096, DType.BF16), (27, 20011, 4100, DType.F16),
                                      (9, 15001, 1500, DType.F32), (32, 30005, 8192, DType.F16)])
 def test_q4_rounds_that_end_unevenly(cuda_device, m, n, k, x):
