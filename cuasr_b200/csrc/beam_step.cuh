@@ -14,6 +14,8 @@
 // an SM); the first three take two to three times as long while the bound is low, and all blocks have theirs at the same time.
 #pragma once
 
+#include <cfloat>
+
 #include "decode_types.cuh"
 
 namespace cuasr_b200 {
@@ -58,7 +60,7 @@ __device__ __forceinline__ float beam_key_logit(unsigned long long key) {
 }
 __device__ __forceinline__ int beam_key_token(unsigned long long key) { return static_cast<int>(~static_cast<unsigned int>(key)); }
 
-// exp(d) for d <= 0: log2(e) in two parts, since one 32-bit factor would shift every term the same way and the sum by
+// exp(d) for d of at most kBeamLag: log2(e) in two parts, since one 32-bit factor would shift every term the same way and the sum by
 // 1e-7 of itself.
 __device__ __forceinline__ float exp_of(float d) {
   const float y = fmaf(d, 1.44269502162933349609375f, d * 1.92596299112661746887e-8f);
@@ -66,6 +68,11 @@ __device__ __forceinline__ float exp_of(float d) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
   return r;
 }
+
+// A thread's sum of exp(logit - ref) is in 64 bits, to which a tile's is added, and `ref` is its maximum of some tile: it is taken
+// anew, and the sum multiplied by a 32-bit exponential, only where the maximum has risen by more than kBeamLag above it, so the roundings of these
+// do not add up however long the row is or slowly its logits rise.
+constexpr float kBeamLag = 16.0f;
 
 // ... of a pair.
 __device__ __forceinline__ uint64_t exp_of_pair(uint64_t d) {
@@ -247,20 +254,27 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
   if (tid == 0)
     for (int s = 0; s < kBeamStages; ++s) copy(v_begin + s * kTile, s);
 
-  float m = -INFINITY, sum = 0.0f;                       // this thread's maximum and sum
+  float m = -INFINITY, ref = -FLT_MAX;                   // this thread's maximum ...
+  double sum = 0.0;                                      // ... and sum of exp(logit - ref)
   float above = -INFINITY, floor = -INFINITY;            // candidates are above `above`; of those found, `keep` reach `floor`
   int held = 0;                                          // candidates of this warp
   unsigned long long* segment = keys + warp * kBeamStride;
   __syncthreads();
+  auto refer = [&] {
+    if (m > ref + kBeamLag) {
+      sum *= exp_of(ref - m);
+      ref = m;
+    }
+  };
   // the few logits outside of whole vectors, one to a lane of the first warp: those in front first, those behind last, so
   // that of equal logits the ones met later always have the higher token
   auto take_one = [&](int at, bool mine) {
-    const float value = mine ? to_float(x[at]) : -INFINITY, m_new = fmaxf(m, value);
+    const float value = mine ? to_float(x[at]) : -INFINITY;
+    m = fmaxf(m, value);
     if constexpr (NORMALISE) {
-      const float ref = m_new == -INFINITY ? 0.0f : m_new;
-      sum = fmaf(sum, exp_of(m - ref), exp_of(value - ref));
+      refer();
+      sum += exp_of(value - ref);
     }
-    m = m_new;
     const unsigned int who = __ballot_sync(0xFFFFFFFFu, value > above);
     if (value > above) segment[held + __popc(who & ((1u << lane) - 1))] = beam_key(value, at);      // there is room for them
     held += __popc(who);
@@ -281,9 +295,9 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
       tops[u] = largest(here[u * kBeamThreads], T());
       top = fmaxf(top, tops[u]);
     }
-    const float m_new = fmaxf(m, top);
+    m = fmaxf(m, top);
     if constexpr (NORMALISE) {
-      const float ref = m_new == -INFINITY ? 0.0f : m_new;
+      refer();
       const uint64_t minus = pack2(-ref, -ref);
       uint64_t s[2] = {0, 0};
 #pragma unroll
@@ -295,9 +309,8 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
       }
       float a, b;
       unpack2(add2(s[0], s[1]), a, b);
-      sum = fmaf(sum, exp_of(m - ref), a + b);
+      sum += a + b;
     }
-    m = m_new;
     if ((tile & (tile - 1)) == 0) {
       const float bound = block_bound(m, p.keep, min((v_end - v_begin + 31) / 32, kBeamWarps), bounds);
       if (bound > floor) {
@@ -384,7 +397,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_part_kernel(co
     if (place[i] >= 0) sorted[from + place[i]] = mine[i];
   if constexpr (NORMALISE) {
     // a thread without a logit above -infinity has a sum of 0, or NaN
-    double s = m == -INFINITY ? static_cast<double>(sum) : static_cast<double>(sum) * static_cast<double>(exp_of(m - all));
+    double s = m == -INFINITY ? sum : sum * static_cast<double>(exp_of(ref - all));
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
     if (lane == 0) sums[warp] = s;

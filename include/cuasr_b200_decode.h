@@ -30,7 +30,8 @@ extern "C" {
  * zeros[j * ld_zeros + k / group], or 8 where `zeros` is NULL.  With x as it is (32-bit values too) and q - zero as the whole
  * number it is, the products are summed by groups in 32 bits, the scale is applied, groups are summed in 32 bits, and Y is rounded
  * once.  Weights at their zero point add exactly nothing; infinities and NaN among the values reach the outputs that the formula
- * gives them to.  Of F32 and BF16 values, bits below 2^-133 and products below 2^-120 may count as zero.
+ * gives them to.  Of F32 and BF16 values, bits below 2^-133 and products below 2^-120 may count as zero;
+ * results below 2^-117 may lose bits.
  * Y must not share bytes with an operand.  The same call gives the same bits every time on one kind of device. */
 typedef struct cuasr_b200_q4_args {
   int32_t dtype_x;      /* CUASR_F32, CUASR_F16 or CUASR_BF16 */
@@ -58,7 +59,7 @@ CUASR_B200_API int cuasr_b200_q4_product(const cuasr_b200_q4_args_t *args);
  *   score[b] + logit[b, v]                              (normalise == 0: the inputs are log-probabilities)
  *   score[b] - log(sum over u of exp(logit[b, u])) + logit[b, v]        (normalise != 0)
  *
- * in 64-bit arithmetic, except for the exponentials (32 bits, summed in 32 bits along a thread's few hundred of them, then in 64).
+ * in 64-bit arithmetic, except for the exponentials (32 bits, summed in 32 bits up to 32 at a time, then in 64).
  * A prefix whose finished byte is not 0 has one continuation: `end_token`, with the prefix's own score.  Values of
  * -infinity and NaN are no continuations (a NaN or +infinity among the logits of a prefix thus ends it where they are
  * normalised).

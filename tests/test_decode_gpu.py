@@ -517,6 +517,36 @@ def test_beam_step_bound_at_the_end_of_a_row(cuda_device, normalise):
         assert wrong.item() == 0
 
 
+@pytest.mark.parametrize("dtype", REALS)
+@pytest.mark.parametrize("shape", ["flat", "rising"])
+def test_beam_step_log_sums_of_long_rows(cuda_device, dtype, shape):
+    """1040 prefixes, so that a block has a whole row, of 2^23 logits: small terms that a sum in 32 bits would not notice one by one but
+    that count together, and logits that rise a little from tile to tile.  All prefixes have the one row (strides of 0)."""
+    batch, beams, vocab, keep = 65, 16, 2 ** 23, 2
+    if shape == "flat":
+        row = torch.full((vocab,), -16.7, device="cuda")
+        row[:4096] = 0
+    else:
+        row = torch.arange(vocab, device="cuda", dtype=torch.float64).mul_(20 / vocab).float()
+    row = row.to(TORCH[dtype])
+    scores = torch.zeros(batch, beams, device="cuda")
+    out = torch.empty(batch, keep, device="cuda")
+    parents, tokens = (torch.empty(batch, keep, device="cuda", dtype=torch.int32) for _ in range(2))
+    op = BeamStep(dtype)
+    args = BeamArguments((batch, beams, vocab, keep), (row, 0, 0), (scores, beams), (out, keep), (parents, keep), (tokens, keep))
+    assert op(args, torch.empty(op.get_workspace_size(args), device="cuda", dtype=torch.uint8)) == Status.kSuccess
+    done()
+    want = (row.double().max() - torch.logsumexp(row.double(), dim=0)).item()
+    # The exponentials and their arguments as in same_choice (the terms lie within 25 of the reference, which a thread's maximum may pass by
+    # 16), twice where the reference is taken anew or the threads' meet, and a tile's sum of up to 32 in 32 bits, ten additions deep; the
+    # score is rounded once.
+    slack = 3 * (2.0 ** -22 + 2.0 ** -18.7) + 10 * 2.0 ** -24
+    assert (out.double() - want).abs().max().item() <= slack + 2.0 ** -24 * 1.001 * abs(want)
+    best = torch.nonzero(row == row.max())[:keep, 0]
+    if best.numel() == keep:
+        assert (parents == 0).all() and (tokens == best.int()).all()
+
+
 def test_beam_step_logits_beyond_32_bit_offsets(cuda_device):
     """Element offsets above 2^31: two searches whose rows lie 2^31 + 16 half-precision numbers apart."""
     far = 2 ** 31 + 16
