@@ -167,12 +167,23 @@ class _DecodeOperator:
             return Status.kErrorInvalidProblem
         return _STATUS[self._can(ctypes.byref(packed))] if self._types_match(args) else Status.kErrorInvalidDataType
 
+    def _check_workspace(self, packed) -> Status:
+        """What the library's call would say to the workspace."""
+        need = self._required_workspace(packed)
+        if need == 0:
+            return Status.kSuccess
+        if not packed.workspace:
+            return Status.kErrorWorkspaceNull
+        if packed.workspace_bytes < need:
+            return Status.kErrorInvalidProblem
+        return Status.kSuccess if packed.workspace % 16 == 0 else Status.kErrorMisalignedOperand
+
     def initialize(self, args, workspace=None, stream=None) -> Status:
         """Checks the call and keeps it for run().  The operator keeps the buffers named in `args` alive."""
         packed = self._pack(args, workspace, stream)
         status = self._check(args, packed)
-        if status is Status.kSuccess and self._required_workspace(packed) > 0 and not packed.workspace:
-            status = Status.kErrorWorkspaceNull
+        if status is Status.kSuccess:
+            status = self._check_workspace(packed)
         if status is Status.kSuccess:
             self._args, self._args_ref, self._keepalive = packed, ctypes.byref(packed), (args, workspace)
         return status

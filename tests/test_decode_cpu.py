@@ -134,6 +134,35 @@ def test_beam_workspace():
         BeamStep(DType.F64)
 
 
+class Room:
+    """A workspace of so many bytes at an address."""
+    def __init__(self, size, at=P):
+        self.size, self.at = size, at
+
+    def numel(self):
+        return self.size
+
+    def element_size(self):
+        return 1
+
+    def data_ptr(self):
+        return self.at
+
+
+def test_beam_initialize_checks_the_workspace():
+    op = BeamStep(DType.F32)
+    need = op.get_workspace_size(beam_args())
+    for room, status in ((Room(need), Status.kSuccess), (Room(need + 1), Status.kSuccess), (Room(need - 1), Status.kErrorInvalidProblem),
+                         (Room(0), Status.kErrorInvalidProblem), (Room(need, P + 8), Status.kErrorMisalignedOperand), (P + 8, Status.kErrorMisalignedOperand),
+                         (Room(need - 1, P + 8), Status.kErrorInvalidProblem), (None, Status.kErrorWorkspaceNull)):
+        fresh = BeamStep(DType.F32)
+        assert fresh.initialize(beam_args(), room) == status
+        if status != Status.kSuccess:
+            assert fresh.run() == Status.kErrorInternal                   # nothing initialised
+            packed = op._pack(beam_args(), room, None)                    # the library says the same
+            assert _lib.load().cuasr_b200_beam_step(ctypes.byref(packed)) == status
+
+
 def reorder_args(states, batch=2, beams=4, keep=4, parents=(P, 4), lengths=None):
     return ReorderArguments((batch, beams, keep), parents, states, lengths)
 
