@@ -88,16 +88,24 @@ class StateView:
     ragged: bool = False
 
 
+def _empty(x) -> bool:
+    """Whether x is a tensor without elements."""
+    return hasattr(x, "numel") and x.numel() == 0
+
+
 def state_view(src, dst=None, position_dim: Optional[int] = None) -> StateView:
     """StateView of a torch tensor whose first two dimensions are batch and beams (dst: the same tensor where it is left
     out).  Without position_dim a row is moved whole; with it, dimension position_dim counts positions and only the
     first lengths[s] of them are moved where the call has lengths.  At most one dimension (or several that lie one behind the
-    other) in front of the positions and contiguous ones behind them can be described; other views raise ValueError."""
+    other) in front of the positions and contiguous ones behind them can be described; other views raise ValueError.  A tensor
+    without elements (a cache without positions yet) is a state of which a call moves nothing."""
     dst = src if dst is None else dst
     if src.dim() < 2 or src.dtype != dst.dtype or src.shape[0] != dst.shape[0] or src.shape[2:] != dst.shape[2:]:
         raise ValueError("src and dst are batch x beams x ... of one type and, but for the beams, one shape")
     if position_dim is not None and not 2 <= position_dim < src.dim():
         raise ValueError("position_dim comes after batch and beams")
+    if _empty(src) and _empty(dst):
+        return StateView(src, dst, (0, 0, 0, 0), (0, 0, 0, 0), 0, 0, 0, position_dim is not None)
     es = src.element_size()
     shape, sides = list(src.shape[2:]), [list(t.stride()[2:]) for t in (src, dst)]
 
@@ -274,8 +282,9 @@ class ReorderStates(_DecodeOperator):
         device = _device((args.ref_parents[0], args.lengths, *(x for s in args.states for x in (s.src, s.dst))))
         if device is None:
             return None
-        states = (_lib.State * max(1, len(args.states)))(*(
+        moved = [s for s in args.states if not (_empty(s.src) and _empty(s.dst))]
+        states = (_lib.State * max(1, len(moved)))(*(
             _lib.State(_ptr(s.src), _ptr(s.dst), *s.src_strides, *s.dst_strides, s.bytes, s.segments, s.positions,
-                       s.ragged and args.lengths is not None, 0) for s in args.states))
-        return _lib.ReorderArgs(*args.problem_size, len(args.states), _ptr(args.ref_parents[0]), args.ref_parents[1],
+                       s.ragged and args.lengths is not None, 0) for s in moved))
+        return _lib.ReorderArgs(*args.problem_size, len(moved), _ptr(args.ref_parents[0]), args.ref_parents[1],
                                 _ptr(args.lengths), states, device, 0, _stream_handle(stream))

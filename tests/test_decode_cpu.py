@@ -225,6 +225,26 @@ def test_nothing_to_reorder_needs_no_device():
     assert ReorderStates()(reorder_args([])) == Status.kSuccess
 
 
+def test_states_without_elements_are_left_out():
+    none = Room(0, 0)
+    op = ReorderStates()
+    assert op(reorder_args([view(src=none, strides=(0, 0, 0, 0), nbytes=0, segments=0, positions=0)] * 2)) == Status.kSuccess
+    packed = op._pack(reorder_args([view(src=none, nbytes=0), view(), view(src=none, positions=0)]), None, None)
+    assert packed.n_states == 1 and packed.states[0].src == P
+    # a side with elements is not nothing, and what is wrong with the call is still wrong
+    assert op.can_implement(reorder_args([view(src=none, dst=P)])) == Status.kErrorInvalidProblem
+    assert op.can_implement(reorder_args([view(src=none)], keep=0)) == Status.kErrorInvalidProblem
+
+
+@pytest.mark.parametrize("shape,position_dim", [((2, 3, 4, 0, 8), 3), ((2, 3, 4, 0, 8), None), ((2, 3, 4, 0, 10, 8), 4), ((2, 3, 0), None), ((2, 3, 0, 4), 2)])
+def test_views_of_states_without_elements(shape, position_dim):
+    x = torch.zeros(shape)
+    v = state_view(x, position_dim=position_dim)
+    assert v.src is x and v.dst is x and v.ragged == (position_dim is not None)
+    with pytest.raises(ValueError):
+        state_view(x, torch.zeros(*shape[:-1], shape[-1] + 1), position_dim)
+
+
 def test_tensors_off_the_gpu_are_refused():
     x = torch.zeros(64, dtype=torch.float16)
     assert Q4Product(DType.F16, group=32).can_implement(q4_args(x=x)) == Status.kErrorInvalidProblem

@@ -664,6 +664,18 @@ def test_reorder_ignores_lengths_out_of_range(cuda_device):
     done()
 
 
+def test_reorder_of_a_cache_without_positions_yet(cuda_device):
+    """As at the first step of a search: the cache has no positions in use, the other states move."""
+    cache = torch.randn(2, 3, 4, 10, 8, generator=gen(33), device="cuda")
+    old, x, parents = cache.clone(), torch.randn(2, 3, 50, generator=gen(34), device="cuda"), parents_of(2, 3, 3, 35)
+    want = x.gather(1, parents.long()[..., None].expand(-1, -1, 50))
+    args = ReorderArguments((2, 3, 3), (parents, 3), [state_view(cache[:, :, :, :0], position_dim=3), state_view(x), state_view(cache[:, :, :0])])
+    before = launch_count()
+    assert ReorderStates()(args) == Status.kSuccess
+    done()
+    assert torch.equal(x, want) and torch.equal(cache, old) and launch_count() - before == 1
+
+
 def test_reorder_beyond_32_bit_offsets(cuda_device):
     """Beams that lie more than 2^32 bytes apart."""
     far = 2 ** 32 + 64
