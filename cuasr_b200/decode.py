@@ -40,6 +40,11 @@ def _device(buffers) -> Optional[int]:
     return found
 
 
+def _held(numbers, bits) -> bool:
+    """Whether signed fields of `bits` bits hold the numbers (ctypes would cut them off)."""
+    return all(-1 << (bits - 1) <= int(x) < 1 << (bits - 1) for x in numbers)
+
+
 _NAMES = {DType.F32: ("float32",), DType.F16: ("float16",), DType.BF16: ("bfloat16",)}
 _BYTES, _FLAGS, _INDEX = ("uint8",), ("uint8", "bool"), ("int32",)
 
@@ -158,7 +163,7 @@ class _DecodeOperator:
         self._keepalive = None
 
     def _pack(self, args, workspace, stream):
-        """The C arguments, or None for buffers that are not on one CUDA device."""
+        """The C arguments, or None for buffers that are not on one CUDA device and for numbers that the C fields do not hold."""
         raise NotImplementedError
 
     def _required_workspace(self, packed) -> int:
@@ -232,7 +237,7 @@ class Q4Product(_DecodeOperator):
         m, n, k = args.problem_size
         refs = (args.ref_X, args.ref_W, args.ref_scales, args.ref_zeros, args.ref_Y)
         device = _device(ref[0] for ref in refs)
-        if device is None:
+        if device is None or not _held((m, n, k, self.group), 32) or not _held((ref[1] for ref in refs), 64):
             return None
         return _lib.Q4Args(self.dtype_x, self.dtype_y, self.dtype_scale, self.group, m, n, k, device,
                            *(field for ref in refs for field in (_ptr(ref[0]), ref[1])), _stream_handle(stream))
@@ -253,7 +258,7 @@ class BeamStep(_DecodeOperator):
     def _pack(self, args: BeamArguments, workspace, stream):
         refs = (args.ref_scores, args.ref_finished, args.ref_out_scores, args.ref_parents, args.ref_tokens)
         device = _device((args.ref_logits[0], workspace, *(ref[0] for ref in refs)))
-        if device is None:
+        if device is None or not _held((*args.problem_size, args.end_token), 32) or not _held((*args.ref_logits[1:], *(ref[1] for ref in refs)), 64):
             return None
         size = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
         packed = _lib.BeamArgs(self.dtype, self.normalise, *args.problem_size, args.end_token, device, _ptr(args.ref_logits[0]),
@@ -280,7 +285,8 @@ class ReorderStates(_DecodeOperator):
 
     def _pack(self, args: ReorderArguments, workspace, stream):
         device = _device((args.ref_parents[0], args.lengths, *(x for s in args.states for x in (s.src, s.dst))))
-        if device is None:
+        if device is None or not _held((*args.problem_size, *(x for s in args.states for x in (s.segments, s.positions))), 32) or \
+                not _held((args.ref_parents[1], *(x for s in args.states for x in (*s.src_strides, *s.dst_strides, s.bytes))), 64):
             return None
         moved = [s for s in args.states if not (_empty(s.src) and _empty(s.dst))]
         states = (_lib.State * max(1, len(moved)))(*(

@@ -134,6 +134,27 @@ def test_beam_workspace():
         BeamStep(DType.F64)
 
 
+WRAP = 2 ** 32                # added to a size, 32 bits do not show it
+
+
+def test_numbers_that_the_fields_do_not_hold_are_refused():
+    bad = Status.kErrorInvalidProblem
+    for change in ({"m": WRAP + 2}, {"n": WRAP + 8}, {"k": WRAP + 64}, {"ldx": 2 ** 64 + 64}, {"ldw": 2 ** 63}, {"z": (P, 2 ** 64 + 2)}):
+        op = Q4Product(DType.F16, group=32)
+        assert op.can_implement(q4_args(**change)) == bad and op.initialize(q4_args(**change)) == bad and op(q4_args(**change)) == bad
+    assert Q4Product(DType.F16, group=WRAP + 32).can_implement(q4_args()) == bad
+    for change in ({"batch": WRAP + 2}, {"beams": WRAP + 3}, {"vocab": WRAP + 10}, {"keep": WRAP + 4}, {"logits": (P, 2 ** 64 + 30, 10)},
+                   {"out": (P, 2 ** 64 + 4)}):
+        op = BeamStep(DType.F32)
+        assert op.can_implement(beam_args(**change)) == bad and op(beam_args(**change), P) == bad and op.get_workspace_size(beam_args(**change)) == 0
+    args = beam_args()
+    args.end_token = WRAP + 2
+    assert BeamStep(DType.F32).can_implement(args) == bad
+    for states, change in (([view()], {"batch": WRAP + 2}), ([view()], {"keep": WRAP + 4}), ([view(positions=WRAP + 2)], {}), ([view(segments=WRAP + 2)], {}),
+                           ([view(nbytes=2 ** 64 + 4)], {}), ([view(strides=(64, 16, 2 ** 64 + 8, 4))], {}), ([view()], {"parents": (P, 2 ** 64 + 4)})):
+        assert ReorderStates().can_implement(reorder_args(states, **change)) == bad
+
+
 class Room:
     """A workspace of so many bytes at an address."""
     def __init__(self, size, at=P):
