@@ -741,6 +741,46 @@ def test_operators_together(cuda_device):
         assert torch.equal(d.cache, torch.where(used, cache[rows, parents], cache)) and torch.equal(d.hidden, hidden[rows, parents])
 
 
+def test_a_search_whose_prefixes_end(cuda_device):
+    """The flags of ended prefixes follow the back-pointers like the other states, and the tokens set them: as in README.md."""
+    batch, beams, vocab, end = 3, 4, 300, 7
+    g = gen(41)
+    table = 2 * torch.randn(batch, vocab, vocab, generator=g, device="cuda")          # logits by the token before
+    table[:, :, end] += 2.0
+    logits = torch.empty(batch, beams, vocab, device="cuda")
+    scores = torch.full((batch, beams), -INF, device="cuda")
+    scores[:, 0] = 0
+    finished = torch.zeros(batch, beams, device="cuda", dtype=torch.uint8)
+    parents, tokens = (torch.zeros(batch, beams, device="cuda", dtype=torch.int32) for _ in range(2))
+    texts = torch.full((batch, beams, 64), -1, device="cuda", dtype=torch.int32)
+    step, reorder, rows = BeamStep(DType.F32), ReorderStates(), torch.arange(batch, device="cuda")[:, None]
+    args = BeamArguments((batch, beams, vocab, beams), (logits, beams * vocab, vocab), (scores, beams), (scores, beams), (parents, beams),
+                         (tokens, beams), (finished, beams), end)
+    workspace = torch.empty(step.get_workspace_size(args), device="cuda", dtype=torch.uint8)
+    assert step.initialize(args, workspace) == Status.kSuccess
+    assert reorder.initialize(ReorderArguments((batch, beams, beams), (parents, beams), [state_view(finished), state_view(texts)])) == Status.kSuccess
+    stream, before = torch.cuda.current_stream(), torch.zeros(batch, beams, device="cuda", dtype=torch.int64)
+    for i in range(64):
+        logits.copy_(table[rows, before])
+        old_scores, old_finished, old_texts = scores.clone(), finished.clone(), texts.clone()
+        want = plain_step(logits, old_scores, beams, True, old_finished, end)
+        for op in (step, reorder):
+            assert op.run(stream) == Status.kSuccess
+        done()
+        same_choice(scores, parents, tokens, *want, True)
+        assert torch.equal(finished, old_finished[rows, parents.long()]) and torch.equal(texts, old_texts[rows, parents.long()])
+        assert (tokens[finished != 0] == end).all()
+        assert torch.equal(scores[finished != 0], old_scores[rows, parents.long()][finished != 0])
+        texts[:, :, i] = tokens
+        finished.logical_or_(tokens == end)
+        before = tokens.long()
+    assert finished.any(dim=1).all()
+    # what follows the end of a prefix is the end again
+    ended_at = (texts == end).int().argmax(dim=2)
+    behind = torch.arange(64, device="cuda") >= ended_at[..., None]
+    assert (texts[behind & (finished != 0)[..., None]] == end).all()
+
+
 def test_captured_steps_replay_like_eager_ones(cuda_device):
     eager, captured = Decoder(22), Decoder(22)
     for _ in range(3):
