@@ -9,8 +9,8 @@
 // below.  The bound comes from the threads' own maxima and is taken again after 1, 2, 4, ... tiles; a row of 16 tiles then has
 // about seven candidates for each that is kept, which every warp collects by itself and which are sorted once, at the row's end.
 //
-// Measured: 64 searches of 16 prefixes over 64000 32-bit logits 58 us, 4.5 TB/s; 32 searches of four over 128000 16-bit logits, a
-// third of the prefixes ended, 19 us.  A block's later tiles pass at the memory's rate (2.3 thousand clocks with seven blocks to
+// Measured: 64 searches of 16 prefixes over 64000 32-bit logits 60 us, 4.4 TB/s; 32 searches of four over 128000 16-bit logits, a
+// third of the prefixes ended, 18.5 us.  A block's later tiles pass at the memory's rate (2.3 thousand clocks with seven blocks to
 // an SM); the first three take two to three times as long while the bound is low, and all blocks have theirs at the same time.
 #pragma once
 
@@ -522,7 +522,7 @@ __host__ __device__ constexpr int beam_merge_scratch(int keep) {
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamParams p) {
   extern __shared__ __align__(16) unsigned char beam_smem[];
   constexpr int kWarps = kMergeThreads / 32;
-  const int lists = p.beams * p.parts, entries = lists * p.keep;                  // at most 1024 + 1036 lists
+  const int lists = p.beams * p.parts, entries = lists * p.keep;                  // at most 1024 lists
   const bool merged = entries <= kBeamMergeMost && lists <= kMergeThreads;
   __shared__ unsigned int bound;
   __shared__ int n_picked;

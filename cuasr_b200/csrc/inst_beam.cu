@@ -7,7 +7,8 @@
 namespace cuasr_b200 {
 
 // As many blocks as the SMs hold at a time, where every part still has a tile and the candidates fit into the merge's shared
-// memory.  (32 searches of four prefixes over 128000 logits of 16 bits: 23 us with eight parts, 25 with six, 29 with three.)
+// memory.  (32 searches of four prefixes over 128000 logits of 16 bits: 23 us with eight
+// parts, 25 with six, 29 with three, when it was chosen; 18.5 with eight now.)
 int beam_parts(const cuasr_b200_beam_args_t& a) {
   const long long rows = static_cast<long long>(a.batch) * a.beams;
   const int tile = kBeamThreads * kBeamVectors * (a.dtype == CUASR_F32 ? 4 : 8);

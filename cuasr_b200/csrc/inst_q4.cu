@@ -44,16 +44,16 @@ Q4Plan plan_q4(int units, int steps, int passes, const Q4Shape& shape, const int
         const double rounds = static_cast<double>(((units + workers - 1) / workers + blocks - 1) / blocks) * passes;
         // In microseconds, from measurements between 1024 x 1024 and 128000 x 4096: a warp's step with all warps at it 1.7 (1.4 where
         // they are eight, 2 for 32 columns), a worker's sums 1.3, a cluster's 2 more; X laid out by a block 0.5 for a step of all its
-        // columns' warps.  Every plan was timed for 24 shapes; the chosen one was the best or within 3 % of it for each.  (One row,
-        // 14336 x 4096: 12.0 with four parts of 16 warps, 12.2 with two of two slices.  Eight rows, 128000 x 4096: 55 with one part, 58
-        // with two, 69 with eight.  Sixteen: 89 with one part or two, 100 with four.  Thirty-two rows, 8192 x 8192: 35 with four slices
-        // of one part, 41 with two of two, 63 with four parts.)
+        // columns' warps.  Every plan was timed for 24 shapes; the chosen one was the best or within 4 % of it for each.  (In
+        // graphs.  One row, 14336 x 4096: 12.4 with four parts of 16 warps, 12.7 with two of two slices.  Eight rows, 128000 x 4096: 57 with
+        // one part, 60 with two, 70 with eight.  Sixteen: 90 with one part, 89 with two, 100 with four.  Thirty-two rows, 8192 x 8192: 32 with
+        // four slices of one part, 37 with two of two, 49 with four parts.)
         const double step = shape.column_tiles == 4 ? 2.0 : warps == 16 ? 1.7 : 1.4;
         const double restaged = plan.panel_steps < slice_steps ? rounds : passes;
         const double cost = rounds * ((slice_steps + parts - 1) / parts * step + (parts > 1 ? 1.3 : 1.0) + (s > 1 ? 2.0 : 0.0)) +
                             restaged * slice_steps * shape.columns * 0.5 / warps;
         plan.grid = blocks * s;
-        // equal plans: the one on more SMs (32 rows, 500 x 1500: 9.3 us with eight parts, 11.6 with two)
+        // equal plans: the one on more SMs (32 rows, 500 x 1500, one slice: 9.3 us with eight parts, 11.6 with two, when it was chosen)
         if (best.smem == 0 || cost < best_cost || (cost == best_cost && plan.grid > best.grid)) {
           best_cost = cost;
           best = plan;

@@ -6,7 +6,7 @@
 
 namespace cuasr_b200 {
 
-// a block has 1 KB of static shared memory and 1 KB that the driver keeps
+// a block has some 300 bytes of static shared memory and 1 KB that the driver keeps
 constexpr int kQ4SmemPerSm = 228 * 1024, kQ4SmemPerBlock = kQ4SmemPerSm - 2048;
 
 struct Q4Launch {

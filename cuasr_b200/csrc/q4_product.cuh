@@ -27,10 +27,12 @@
 // Where there are few weight rows for the SMs, or X is too large for a block's shared memory, the blocks of a cluster share k, and
 // their sums meet through distributed shared memory.
 //
-// What bounds it: for large n the instructions of a step (eight rows, 128000 x 4096: 55 us, 5.0 TB/s; the same pipeline without the
-// products 45 us); with more columns of X the chain of a warp's instructions, neither their number, nor the products (a third of the
+// What bounds it: for large n the instructions of a step (eight rows, 128000 x 4096, weights that are not in L2: 65 us, 4.2 TB/s; the
+// issue slots are 57 % full, the pipe that does the ANDs 49 %); with more columns of X the chain of a warp's instructions (32 rows, 8192 x 8192:
+// 32.6 us), neither their number, nor the products (a third of the
 // rate of mma.sync), nor the reads of X, each of which was taken out in a trial without a gain; for small n what precedes the products
-// (the launch, X laid out: 2 to 8 us).  Tried and slower: three stages, one box of 128 bytes instead of two of 64, clusters of eight
+// (the launch, X laid out: 2 to 8 us).  Pairs of times in this file compare two choices as the kernel was when one was made; times change by
+// 5 % either way with what has been mended since.  Tried and slower: three stages, one box of 128 bytes instead of two of 64, clusters of eight
 // (15 run at a time: 32 rows, 8192 x 8192 57 us instead of 35), more loads of X in flight (the registers: 57 us
 // with four of a warp instead of two), all products of one pair before those of the other (63 instead of 61).
 #pragma once
@@ -325,7 +327,7 @@ q4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Q4Par
   const int end = static_cast<int>(static_cast<long long>(all_steps) * (slice + 1) / p.slices);
   const bool one_panel = end - begin <= p.panel_steps;
   // In more than one round neighbouring units are in different blocks, so that the last, which need not be full, leaves every SM as
-  // much to do (eight rows, 128000 x 4096: 57 us instead of 60.7); in one round in the same block (32 rows, 8192 x 8192: 34.9 us
+  // much to do (eight rows, 128000 x 4096 in a graph: 57 us instead of 60.7); in one round in the same block (32 rows, 8192 x 8192: 34.9 us
   // instead of 36.3).
   const int clusters = static_cast<int>(gridDim.x) / p.slices, cluster = static_cast<int>(blockIdx.x) / p.slices;
   const int workers = clusters * workers_here, rounds = (p.units + workers - 1) / workers;
