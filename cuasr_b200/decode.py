@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import struct
 from typing import Any, Optional, Sequence, Tuple
 
 from . import _lib
@@ -40,9 +41,9 @@ def _device(buffers) -> Optional[int]:
     return found
 
 
-def _held(numbers, bits) -> bool:
-    """Whether signed fields of `bits` bits hold the numbers (ctypes would cut them off)."""
-    return all(-1 << (bits - 1) <= int(x) < 1 << (bits - 1) for x in numbers)
+# the C arguments' layouts: a number that its field does not hold is an error here, where ctypes would cut it off
+_PACK = {kind: struct.Struct(layout).pack for kind, layout in (
+    (_lib.Q4Args, "8i" + 5 * "Qq" + "Q"), (_lib.BeamArgs, "8iQqq" + 5 * "Qq" + "QNQ"), (_lib.State, "QQ8qq4i"), (_lib.ReorderArgs, "4iQqQQ2iQ"))}
 
 
 _NAMES = {DType.F32: ("float32",), DType.F16: ("float16",), DType.BF16: ("bfloat16",)}
@@ -163,7 +164,14 @@ class _DecodeOperator:
         self._keepalive = None
 
     def _pack(self, args, workspace, stream):
-        """The C arguments, or None for buffers that are not on one CUDA device and for numbers that the C fields do not hold."""
+        try:
+            return self._packed(args, workspace, stream)
+        except struct.error:
+            return None
+
+    def _packed(self, args, workspace, stream):
+        """The C arguments, or None for buffers that are not on one CUDA device; struct.error for numbers that the C fields
+        do not hold."""
         raise NotImplementedError
 
     def _required_workspace(self, packed) -> int:
@@ -233,14 +241,15 @@ class Q4Product(_DecodeOperator):
         return _typed((args.ref_X[0], _NAMES[self.dtype_x]), (args.ref_W[0], _BYTES), (args.ref_scales[0], _NAMES[self.dtype_scale]),
                       (args.ref_zeros[0], _BYTES), (args.ref_Y[0], _NAMES[self.dtype_y]))
 
-    def _pack(self, args: Q4Arguments, workspace, stream):
+    def _packed(self, args: Q4Arguments, workspace, stream):
         m, n, k = args.problem_size
         refs = (args.ref_X, args.ref_W, args.ref_scales, args.ref_zeros, args.ref_Y)
         device = _device(ref[0] for ref in refs)
-        if device is None or not _held((m, n, k, self.group), 32) or not _held((ref[1] for ref in refs), 64):
+        if device is None:
             return None
-        return _lib.Q4Args(self.dtype_x, self.dtype_y, self.dtype_scale, self.group, m, n, k, device,
-                           *(field for ref in refs for field in (_ptr(ref[0]), ref[1])), _stream_handle(stream))
+        return _lib.Q4Args.from_buffer_copy(_PACK[_lib.Q4Args](
+            self.dtype_x, self.dtype_y, self.dtype_scale, self.group, m, n, k, device,
+            *(field for ref in refs for field in (_ptr(ref[0]), ref[1])), _stream_handle(stream)))
 
 
 class BeamStep(_DecodeOperator):
@@ -255,15 +264,15 @@ class BeamStep(_DecodeOperator):
         return _typed((args.ref_logits[0], _NAMES[self.dtype]), (args.ref_scores[0], _NAMES[DType.F32]), (args.ref_finished[0], _FLAGS),
                       (args.ref_out_scores[0], _NAMES[DType.F32]), (args.ref_parents[0], _INDEX), (args.ref_tokens[0], _INDEX))
 
-    def _pack(self, args: BeamArguments, workspace, stream):
+    def _packed(self, args: BeamArguments, workspace, stream):
         refs = (args.ref_scores, args.ref_finished, args.ref_out_scores, args.ref_parents, args.ref_tokens)
         device = _device((args.ref_logits[0], workspace, *(ref[0] for ref in refs)))
-        if device is None or not _held((*args.problem_size, args.end_token), 32) or not _held((*args.ref_logits[1:], *(ref[1] for ref in refs)), 64):
+        if device is None:
             return None
         size = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
-        packed = _lib.BeamArgs(self.dtype, self.normalise, *args.problem_size, args.end_token, device, _ptr(args.ref_logits[0]),
-                               *args.ref_logits[1:], *(field for ref in refs for field in (_ptr(ref[0]), ref[1])),
-                               _ptr(workspace), size, _stream_handle(stream))
+        packed = _lib.BeamArgs.from_buffer_copy(_PACK[_lib.BeamArgs](
+            self.dtype, self.normalise, *args.problem_size, args.end_token, device, _ptr(args.ref_logits[0]), *args.ref_logits[1:],
+            *(field for ref in refs for field in (_ptr(ref[0]), ref[1])), _ptr(workspace), size, _stream_handle(stream)))
         if workspace is not None and not hasattr(workspace, "numel"):       # an address: as large as was asked for
             packed.workspace_bytes = self._required_workspace(packed)
         return packed
@@ -283,14 +292,16 @@ class ReorderStates(_DecodeOperator):
     def _types_match(self, args: ReorderArguments) -> bool:
         return _typed((args.ref_parents[0], _INDEX), (args.lengths, _INDEX))
 
-    def _pack(self, args: ReorderArguments, workspace, stream):
+    def _packed(self, args: ReorderArguments, workspace, stream):
         device = _device((args.ref_parents[0], args.lengths, *(x for s in args.states for x in (s.src, s.dst))))
-        if device is None or not _held((*args.problem_size, *(x for s in args.states for x in (s.segments, s.positions))), 32) or \
-                not _held((args.ref_parents[1], *(x for s in args.states for x in (*s.src_strides, *s.dst_strides, s.bytes))), 64):
+        if device is None:
             return None
-        moved = [s for s in args.states if not (_empty(s.src) and _empty(s.dst))]
-        states = (_lib.State * max(1, len(moved)))(*(
-            _lib.State(_ptr(s.src), _ptr(s.dst), *s.src_strides, *s.dst_strides, s.bytes, s.segments, s.positions,
-                       s.ragged and args.lengths is not None, 0) for s in moved))
-        return _lib.ReorderArgs(*args.problem_size, len(moved), _ptr(args.ref_parents[0]), args.ref_parents[1],
-                                _ptr(args.lengths), states, device, 0, _stream_handle(stream))
+        pack, some = _PACK[_lib.State], args.lengths is not None
+        moved = [pack(_ptr(s.src), _ptr(s.dst), *s.src_strides, *s.dst_strides, s.bytes, s.segments, s.positions, bool(s.ragged and some), 0)
+                 for s in args.states if not (_empty(s.src) and _empty(s.dst))]
+        states = (_lib.State * max(1, len(moved))).from_buffer_copy(b"".join(moved) or bytes(ctypes.sizeof(_lib.State)))
+        packed = _lib.ReorderArgs.from_buffer_copy(_PACK[_lib.ReorderArgs](
+            *args.problem_size, len(moved), _ptr(args.ref_parents[0]), args.ref_parents[1], _ptr(args.lengths), ctypes.addressof(states), device, 0,
+            _stream_handle(stream)))
+        packed.kept = states         # as long as the pointer to them
+        return packed

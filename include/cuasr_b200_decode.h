@@ -28,8 +28,8 @@ extern "C" {
  *
  * q[j, k] is the low (k even) or high (k odd) half of the byte W[j * ldw + k / 2]; zero is the low half of
  * zeros[j * ld_zeros + k / group], or 8 where `zeros` is NULL.  With x as it is (32-bit values too) and q - zero as the whole
- * number it is, the products are summed by groups in 32 bits, the scale is applied, groups are summed in 32 bits, and Y is rounded
- * once.  Weights at their zero point add exactly nothing; infinities and NaN among the values reach the outputs that the formula
+ * number it is, the products are summed in 32 bits by groups, of longer ones by 128, the scale is applied, these are summed in 32 bits, and Y is
+ * rounded once.  Weights at their zero point add exactly nothing; infinities and NaN among the values reach the outputs that the formula
  * gives them to.  Of F32 and BF16 values, bits below 2^-133 and products below 2^-120 may count as zero;
  * results below 2^-117 may lose bits.
  * Y must not share bytes with an operand.  The same call gives the same bits every time on one kind of device. */
